@@ -10,7 +10,7 @@ from .config import (ModelSpec, PartSpec, Qwen3Config, BusavikConfig, FimudraCon
 from .errors import CacheError, ConfigError, InferError, KernelError, WeightsError
 from .weights import SafeTensorsFolder, write_random_model, write_safetensors
 from .engine import DecoderModel, Engine, Entry, Runtime
-from .sampling import Sampling, sampling_from_config
+from .sampling import Sampling, Scores, sampling_from_config, token_scores
 from .client import LlmClient
 
 __all__ = ["ModelSpec", "PartSpec", "Qwen3Config", "BusavikConfig", "FimudraConfig", "SezopelConfig", "LaralixConfig",
@@ -18,4 +18,4 @@ __all__ = ["ModelSpec", "PartSpec", "Qwen3Config", "BusavikConfig", "FimudraConf
            "config_of_folder", "register_architecture", "CacheError", "ConfigError",
            "InferError", "KernelError", "WeightsError", "SafeTensorsFolder",
            "write_random_model", "write_safetensors", "DecoderModel", "Engine", "Entry",
-           "Runtime", "Sampling", "sampling_from_config", "LlmClient"]
+           "Runtime", "Sampling", "Scores", "sampling_from_config", "token_scores", "LlmClient"]

@@ -44,6 +44,16 @@ class FreeList:
         self._held[i] = True
         return i
 
+    def take_many(self, n: int) -> List[int]:
+        """``n`` of them at once, those that ``n`` calls of ``take`` would hand out."""
+        if n > len(self._free):
+            raise CacheError(f"no {n} free {self.what}s ({len(self._free)} of {self.count})")
+        got = self._free[len(self._free) - n:][::-1]
+        del self._free[len(self._free) - n:]
+        for i in got:
+            self._held[i] = True
+        return got
+
     def give(self, i: int) -> None:
         if not 0 <= i < self.count:
             raise CacheError(f"{self.what} {i} does not exist (there are {self.count})")
@@ -159,27 +169,44 @@ class CacheBook:
         ``requests = [(slot, new_length)]``. All or nothing: if a pool runs out, nothing is
         mapped and ``CacheError`` is raised. Returns, per group, the new table entries
         ``(slot, entry, page)``."""
+        out = []
+        for held, pages in self.grow(requests):
+            entries, at = [], 0
+            for (slot, _), (h, n) in zip(requests, held):
+                entries += [(slot, h + j, page) for j, page in enumerate(pages[at:at + n])]
+                at += n
+            out.append(entries)
+        return out
+
+    def grow(self, requests: List[Tuple[int, int]]) -> List[Tuple[List[Tuple[int, int]], List[int]]]:
+        """``reserve`` that names no entry by itself: per group ``(held, pages)``, for every request
+        the pages that its slot held before and how many it received, and all received pages in that
+        order."""
         for slot, new_length in requests:
             self.check_open(slot)
             if new_length > self.max_context:
                 raise CacheError(
                     f"slot {slot}: {new_length} positions exceed the context of {self.max_context}")
-        want = [0] * len(self.plans)
-        for slot, new_length in requests:
-            for g, n in enumerate(self.missing(slot, new_length)):
-                want[g] += n
         for g, pool in enumerate(self.pools):
-            if want[g] > pool.free:
+            want = 0
+            for slot, new_length in requests:
+                want += max(0, self.entries_needed(g, new_length) - len(self.pages[g][slot]))
+            if want > pool.free:
                 raise CacheError(
-                    f"the cache is full: {want[g]} more pages needed, {pool.free} of "
+                    f"the cache is full: {want} more pages needed, {pool.free} of "
                     f"{pool.count} free")
-        out: List[List[Tuple[int, int, int]]] = [[] for _ in self.plans]
-        for slot, new_length in requests:
-            for g, n in enumerate(self.missing(slot, new_length)):
-                for _ in range(n):
-                    page = self.pools[g].take()
-                    self.pages[g][slot].append(page)
-                    out[g].append((slot, len(self.pages[g][slot]) - 1, page))
+        out = []
+        for g, pool in enumerate(self.pools):
+            held, pages = [], []
+            for slot, new_length in requests:
+                mine = self.pages[g][slot]
+                n = max(0, self.entries_needed(g, new_length) - len(mine))
+                held.append((len(mine), n))
+                if n:
+                    got = pool.take_many(n)
+                    mine += got
+                    pages += got
+            out.append((held, pages))
         for slot, new_length in requests:
             self.high[slot] = max(self.high[slot], new_length)
         return out

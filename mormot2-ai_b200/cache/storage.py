@@ -14,8 +14,12 @@ from typing import Dict, List, Optional, Tuple
 import numpy as np
 import torch
 
+from .. import kernels as K
 from .guards import Guards, alloc
 from .pages import PAGE, CacheBook, GroupPlan
+
+# Entries of a page table that are copied as whole rows; more are written by a kernel.
+MAP_ROWS = 8192
 
 
 @dataclass
@@ -101,6 +105,30 @@ class CacheStorage:
             host.numpy()[where[:, 0], where[:, 1]] = where[:, 2]
             lo, hi = int(where[:, 0].min()), int(where[:, 0].max())
             self.tables[g][lo:hi + 1].copy_(host[lo:hi + 1], non_blocking=True)
+
+    def map_grown(self, slots: List[int], past: List[int], new: List[int], grown) -> None:
+        """``map_pages`` for what ``CacheBook.grow`` returned for distinct ``slots`` that held
+        ``past`` positions and grow by ``new``. Where whole rows of the tables would be many bytes,
+        the lengths and the pages alone are copied and a kernel writes the entries."""
+        for g, (held, pages) in enumerate(grown):
+            if not pages:
+                continue
+            host = self.tables_host[g].numpy()
+            at, lo, hi = 0, len(host), 0
+            for slot, (h, n) in zip(slots, held):
+                if n:
+                    host[slot, h:h + n] = pages[at:at + n]
+                    at += n
+                    lo, hi = min(lo, slot), max(hi, slot)
+            if (hi + 1 - lo) * host.shape[1] <= MAP_ROWS:
+                self.tables[g][lo:hi + 1].copy_(self.tables_host[g][lo:hi + 1], non_blocking=True)
+                continue
+            B = len(slots)
+            lists = np.array([*slots, *past, *new, *(h for h, _ in held), *pages], dtype=np.int32)
+            # (pageable: staged before the copy returns)
+            dev = torch.from_numpy(lists).to(self.tables[g].device, non_blocking=True)
+            K.map_pages(self.tables[g], dev[:B], dev[B:2 * B], dev[2 * B:3 * B], dev[3 * B:4 * B],
+                        dev[4 * B:], self.plans[g].ring_pages)
 
     def table_faults(self, book: CacheBook) -> List[str]:
         """Compares the page tables on the device with the bookkeeping: every entry that a

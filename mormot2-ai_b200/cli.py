@@ -7,6 +7,7 @@ and answers are token ids: tokenizers are not part of this library.
 
     python -m mormot2_ai_b200 llm-bench <folder> [prompt tokens=200] [new tokens=32] [bf16|f32]
     python -m mormot2_ai_b200 llm-quickstart <folder> [ids "5,17,3;9,2"] [bf16|f32] [options]
+    python -m mormot2_ai_b200 llm-score <folder> <ids "5,17,3;9,2"> [bf16|f32] [--top k]
     python -m mormot2_ai_b200 random-model <out folder> <config.json> [seed=0]
 """
 from __future__ import annotations
@@ -124,15 +125,50 @@ def llm_quickstart(argv: List[str]) -> int:
     ap.add_argument("--seed", type=int, default=None)
     ap.add_argument("--stop", type=int, action="append", default=None,
                     help="a stop token id (repeatable); default: the model's eos_token_id")
+    ap.add_argument("--logprobs", type=int, default=None,
+                    help="also print every new token's log probability, the entropy it was chosen "
+                         "at and so many (0 to 32) alternatives")
     a = ap.parse_args(argv)
     from .client import LlmClient
     prompts = [[int(t) for t in part.split(",") if t.strip()] for part in a.ids.split(";")]
     client = LlmClient(a.folder, dtype=_dtype(a.weights), max_context=a.max_context,
                        max_batch=max(1, len(prompts)))
     out = client.generate(prompts, max_tokens=a.max_tokens, temperature=a.temperature,
-                          top_k=a.top_k, top_p=a.top_p, min_p=a.min_p, seed=a.seed, stop=a.stop)
-    for tokens in out:
-        print(",".join(str(t) for t in tokens))
+                          top_k=a.top_k, top_p=a.top_p, min_p=a.min_p, seed=a.seed, stop=a.stop,
+                          logprobs=a.logprobs)
+    for answer in out:
+        print(",".join(str(t) for t in (answer if a.logprobs is None else answer.tokens)))
+        if a.logprobs is not None:
+            _print_scores(answer.tokens, answer.scores)
+    return 0
+
+
+def _print_scores(tokens, scores) -> None:
+    for token, s in zip(tokens, scores):
+        rest = " ".join(f"{i}:{p:.4f}" for i, p in s.alternatives)
+        print(f"  {token:>8} {s.logprob:10.4f}  entropy {s.entropy:8.4f}  {rest}".rstrip())
+
+
+def llm_score(argv: List[str]) -> int:
+    """Says how probable given texts (token ids) are: log probability and perplexity of each, and
+    with --top the log probability, entropy and alternatives of every token."""
+    ap = argparse.ArgumentParser(prog="llm-score", description=llm_score.__doc__)
+    ap.add_argument("folder")
+    ap.add_argument("ids", help="texts as token ids: \"5,17,3;9,2\" (';' between texts)")
+    ap.add_argument("weights", nargs="?", default="bf16", help="bf16 (default) | f32")
+    ap.add_argument("--top", type=int, default=None,
+                    help="print every token's scores with so many (0 to 32) alternatives")
+    ap.add_argument("--max-context", type=int, default=None)
+    a = ap.parse_args(argv)
+    from .client import LlmClient
+    texts = [[int(t) for t in part.split(",") if t.strip()] for part in a.ids.split(";")]
+    client = LlmClient(a.folder, dtype=_dtype(a.weights), max_context=a.max_context,
+                       max_batch=max(1, len(texts)))
+    for text, s in zip(texts, client.score(texts, a.top or 0)):
+        print(f"{len(s.tokens)} tokens scored: log probability {s.logprob:.4f}, "
+              f"perplexity {s.perplexity:.4f}")
+        if a.top is not None:
+            _print_scores(text[1:], s.tokens)
     return 0
 
 
@@ -156,7 +192,8 @@ def random_model(argv: List[str]) -> int:
     return 0
 
 
-COMMANDS = {"llm-bench": llm_bench, "llm-quickstart": llm_quickstart, "random-model": random_model}
+COMMANDS = {"llm-bench": llm_bench, "llm-quickstart": llm_quickstart, "llm-score": llm_score,
+            "random-model": random_model}
 
 
 def main(argv: List[str] = None) -> int:

@@ -13,15 +13,17 @@ generation_config.json as ``InferSamplingFromConfig`` does), ``max_tokens`` (``M
 """
 from __future__ import annotations
 
+import math
 import os
 import random
-from dataclasses import replace
+from dataclasses import dataclass, replace
 from typing import Iterable, List, Optional, Sequence
 
 from .config.registry import read_config_json
-from .engine.engine import Engine
-from .engine.generate import EngineStepper, Outcome, Request, generate
+from .engine.engine import Engine, Entry
+from .engine.generate import EngineStepper, Outcome, Request, generate, plan_batches
 from .errors import InferError
+from .sampling.scores import TokenScore
 from .sampling.settings import Sampling, sampling_from_config
 
 
@@ -36,6 +38,25 @@ def _stop_ids(folder: str) -> List[int]:
             if isinstance(eos, list) and eos:
                 return [int(e) for e in eos]
     return []
+
+
+@dataclass
+class TextScore:
+    """The scores of a text: one ``TokenScore`` for every token but the first."""
+    tokens: List[TokenScore]
+
+    @property
+    def logprob(self) -> float:
+        """The log probability of the whole text after its first token."""
+        return math.fsum(t.logprob for t in self.tokens)
+
+    @property
+    def perplexity(self) -> float:
+        """exp of the mean negative log probability a token (1 for a text of one token)."""
+        if not self.tokens:
+            return 1.0
+        mean = -self.logprob / len(self.tokens)
+        return math.inf if mean > 709.0 else math.exp(mean)
 
 
 class LlmClient:
@@ -73,9 +94,12 @@ class LlmClient:
                  temperature: float = -1.0, top_k: Optional[int] = None,
                  top_p: Optional[float] = None, min_p: Optional[float] = None,
                  seed: Optional[int] = None, stop: Optional[Iterable[int]] = None,
-                 details: bool = False):
+                 details: bool = False, logprobs: Optional[int] = None):
         """New token ids of every prompt (the stop token included when one ended it). Sequence
-        i draws from the stream of ``seed + i``. ``details``: ``Outcome`` objects instead."""
+        i draws from the stream of ``seed + i``. ``details``: ``Outcome`` objects instead.
+        ``logprobs`` (0 to 32): ``Outcome`` objects whose ``scores`` hold, for every new token, its
+        log probability, the entropy of what it was chosen from and so many alternatives; they are
+        the model's own, before temperature and filters."""
         s = self.sampling
         s = replace(s, temperature=temperature if temperature >= 0 else s.temperature,
                     top_k=s.top_k if top_k is None else top_k,
@@ -85,9 +109,47 @@ class LlmClient:
         stops = set(self.stop if stop is None else stop)
         cap = self.max_tokens if max_tokens is None else max_tokens
         requests = [Request(list(p), cap, stops, base + i) for i, p in enumerate(prompts)]
-        self.stepper = EngineStepper(self.engine, s, self.vocab_limit, self.max_batch)
+        self.stepper = EngineStepper(self.engine, s, self.vocab_limit, self.max_batch, logprobs)
         outcomes = generate(self.stepper, requests)
-        return outcomes if details else [o.tokens for o in outcomes]
+        return outcomes if details or logprobs is not None else [o.tokens for o in outcomes]
+
+    def score(self, sequences: Sequence[Sequence[int]], top: int = 0) -> List[TextScore]:
+        """What the model says of given texts: for every token of a sequence but its first, the
+        log probability after the tokens before it, the entropy there and the ``top`` (0 to 32) most
+        probable alternatives. Sequences run together as the cache allows."""
+        texts = [[int(t) for t in s] for s in sequences]
+        for i, t in enumerate(texts):
+            if not t:
+                raise InferError(f"sequence {i}: empty")
+            if len(t) > self.max_context + 1:       # the last token is not fed
+                raise InferError(f"sequence {i}: {len(t)} tokens exceed the context of "
+                                 f"{self.max_context} and one")
+            bad = [a for a in t if not 0 <= a < self.engine.vocab_size]
+            if bad:
+                raise InferError(f"sequence {i}: token {bad[0]} is outside the vocabulary of "
+                                 f"{self.engine.vocab_size}")
+        out = [TextScore([]) for _ in texts]
+        fed = [i for i, t in enumerate(texts) if len(t) > 1]
+        pools = [(p.n_pages, p.ring_pages) for p in self.engine.plans]
+        requests = [Request(texts[i][:-1], 1) for i in fed]
+        for batch in plan_batches(requests, self.max_batch, pools):
+            slots: List[int] = []
+            try:
+                for _ in batch:
+                    slots.append(self.engine.open())
+                got = self.engine.score(
+                    [Entry(slot, requests[k].prompt, given=texts[fed[k]][1:])
+                     for slot, k in zip(slots, batch)], top, self.vocab_limit).on_host()
+                self.engine.rt.check()
+            finally:
+                for slot in slots:
+                    self.engine.close(slot)
+            at = 0
+            for k in batch:
+                n = len(requests[k].prompt)
+                out[fed[k]].tokens = got[at:at + n]
+                at += n
+        return out
 
     def greedy(self, prompt: Sequence[int], max_new: int, stop: Iterable[int] = ()) -> List[int]:
         """Greedy decoding of one prompt (``TDecoderModel.Greedy``, ``decoder.pas:3390-3426``)."""

@@ -45,6 +45,8 @@ SOURCES = {
     "gemm_split": "gemm_split.cu",
     "attention_simt": "attention_simt.cu",
     "sampling": "sampling.cu",
+    "scores": "scores.cu",
+    "step_index": "step_index.cu",
     "gemm_tc": "gemm_tc.cu",
     "attention_mma": "attention_mma.cu",
     "attention_tc": "attention_tc.cu",
@@ -71,6 +73,7 @@ EXTRA_HEADERS = {"gemm_tc": ["tc_common.cuh"],
                                     "tc_common.cuh"],
                  "attention_tc": ["attention_tc.cuh", "tc_common.cuh"],
                  "attention_diff_tc": ["attention_tc.cuh", "tc_common.cuh"],
+                 "scores": ["scores.cuh"],
                  "latent": ["mma_common.cuh", "mma_tile.cuh"],
                  "moe": ["mma_common.cuh", "moe_act.cuh"],
                  "moe_tc": ["tc_common.cuh", "moe_act.cuh"],

@@ -3,7 +3,8 @@
 The tokens of all sequences are packed one after another (no padding); per token the index of
 its sequence and its position, per sequence its slot, its first packed row and how many
 positions it held before. Parts and kernels read only this. All index arrays live in one
-device buffer that is filled by one copy from pinned host memory.
+device buffer that is filled by one copy from pinned host memory and, in a step of many tokens, by
+a kernel that works out from the sequences' lengths what follows from them.
 """
 from __future__ import annotations
 
@@ -13,6 +14,7 @@ from typing import List, Sequence, Tuple
 import numpy as np
 import torch
 
+from .. import kernels as K
 from ..errors import InferError
 
 
@@ -63,6 +65,7 @@ class StepBuffers:
         self.dev = alloc(guards, "step index arrays", (self.size,), torch.int32, device)
         self.copied = torch.cuda.Event()
         self.in_flight = False
+        self.copied_bytes = 0       # of the last fill
         self.views = {}
 
     def fill(self, seqs: Sequence[Tuple[int, int, Sequence[int], Sequence[int]]],
@@ -118,25 +121,8 @@ class StepBuffers:
             self.host_np[:total] = (ids + seq + pos + tslot + [s[0] for s in seqs] + starts
                                     + [s[1] for s in seqs] + wants)
         else:
-            starts = np.zeros(B + 1, dtype=np.int64)
-            np.cumsum(n_new, out=starts[1:])
-            flat = self.host_np[:total]
-            at = 0
-            for b, (slot, past, tokens, want) in enumerate(seqs):
-                n, lo = n_new[b], int(starts[b])
-                flat[o_ids + lo:o_ids + lo + n] = tokens
-                flat[o_seq + lo:o_seq + lo + n] = b
-                flat[o_pos + lo:o_pos + lo + n] = np.arange(past, past + n, dtype=np.int32)
-                flat[o_tslot + lo:o_tslot + lo + n] = slot
-                flat[o_slot + b] = slot
-                flat[o_past + b] = past
-                if len(want):
-                    flat[o_want + at:o_want + at + len(want)] = np.asarray(want, dtype=np.int64) + lo
-                    at += len(want)
-            flat[o_start:o_start + B + 1] = starts
-        self.dev[:total].copy_(self.host[:total], non_blocking=True)
-        self.copied.record()
-        self.in_flight = True
+            return self._fill_many(seqs, n_new, T, n_want)
+        self._copy(total)
         # the device views depend on the counts only: made once per shape of step
         views = self.views.get((T, B, n_want, o_entry))
         if views is None:
@@ -147,8 +133,56 @@ class StepBuffers:
             views += (views[4] if o_entry == o_slot else d[o_entry:o_entry + B],)
             if len(self.views) < 4096:
                 self.views[(T, B, n_want, o_entry)] = views
+        return self._context(seqs, n_new, T, n_want, views)
+
+    def _copy(self, total: int) -> None:
+        self.dev[:total].copy_(self.host[:total], non_blocking=True)
+        self.copied.record()
+        self.in_flight = True
+        self.copied_bytes = 4 * total
+
+    def _fill_many(self, seqs, n_new: List[int], T: int, n_want: int) -> StepContext:
+        """A step of many tokens: ids, lengths and wanted rows are copied, and what follows from the
+        lengths (a token's sequence, position and slot, a sequence's first row) is worked out on the
+        device. On the host these arrays cost ten microseconds a sequence and four times the bytes."""
+        B = len(seqs)
+        o_want, o_slot = T, T + n_want
+        o_past, o_new, o_start = o_slot + B, o_slot + 2 * B, o_slot + 3 * B
+        o_seq = o_start + B + 1
+        o_pos, o_tslot = o_seq + T, o_seq + 2 * T
+        flat = self.host_np
+        np.concatenate([s[2] for s in seqs], out=flat[:T], casting="unsafe")
+        flat[o_slot:o_past] = [s[0] for s in seqs]
+        flat[o_past:o_new] = [s[1] for s in seqs]
+        flat[o_new:o_start] = n_new
+        at, lo = o_want, 0
+        for s, n in zip(seqs, n_new):
+            k = len(s[3])
+            if k == 1:
+                flat[at] = lo + s[3][0]
+            elif k:
+                np.add(s[3], lo, out=flat[at:at + k], casting="unsafe")
+            at += k
+            lo += n
+        views = self.views.get((T, B, n_want, -1))
+        if views is None:
+            d = self.dev
+            views = (d[:T], d[o_seq:o_pos], d[o_pos:o_tslot], d[o_tslot:o_tslot + T],
+                     d[o_slot:o_past], d[o_start:o_seq], d[o_past:o_new], d[o_want:o_slot],
+                     d[o_slot:o_past], d[o_new:o_start])
+            if len(self.views) < 4096:
+                self.views[(T, B, n_want, -1)] = views
+        # The ids are copied last: a kernel may read a step's arrays ahead of its wait for the kernel
+        # before it, so that must be no kernel that writes them.
+        self.dev[o_slot:o_start].copy_(self.host[o_slot:o_start], non_blocking=True)
+        K.step_index(views[4], views[6], views[9], views[5], views[1], views[2], views[3])
+        self._copy(o_slot)
+        self.copied_bytes = 4 * o_start
+        return self._context(seqs, n_new, T, n_want, views)
+
+    def _context(self, seqs, n_new: List[int], T: int, n_want: int, views) -> StepContext:
         return StepContext(
-            T=T, B=B, tok_ids=views[0], tok_seq=views[1], tok_pos=views[2], tok_slot=views[3],
+            T=T, B=len(seqs), tok_ids=views[0], tok_seq=views[1], tok_pos=views[2], tok_slot=views[3],
             seq_slot=views[4], seq_start=views[5], seq_past=views[6], want_rows=views[7],
             n_want=n_want, entry_slots=views[8], max_new=max(n_new),
             max_len=max(s[1] + len(s[2]) for s in seqs), decode=max(n_new) == 1,

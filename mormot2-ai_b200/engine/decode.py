@@ -25,6 +25,7 @@ import torch
 
 from .. import kernels as K
 from ..errors import InferError
+from ..sampling.scores import Scores, TokenScore, token_scores
 
 
 class DecodeRun:
@@ -39,8 +40,9 @@ class DecodeRun:
 
     def __init__(self, engine, ctx, slots: List[int], tokens: List[int], max_steps: int,
                  sampler, sampling, vocab_limit: Optional[int], history: bool,
-                 order: Optional[List[int]] = None):
-        # ``order[j]``: which of ``slots`` row j of ``ctx`` (and of every step's picks) is
+                 order: Optional[List[int]] = None, top: Optional[int] = None):
+        # ``order[j]``: which of ``slots`` row j of ``ctx`` (and of every step's picks) is.
+        # ``top``: every pick is scored too, with so many alternatives (None: it is not)
         self.engine, self.ctx, self.slots = engine, ctx, slots
         self.order = None if order is None or order == sorted(order) else list(order)
         self.first_tokens = tokens
@@ -57,6 +59,16 @@ class DecodeRun:
         self.history = (torch.empty((max_steps, ctx.B), dtype=torch.int32, device=rt.device)
                         if history else None)
         self.d2h_bytes = 0
+        self.scores = None
+        self.last_scores: List[TokenScore] = []     # of the step read last, in the order of the slots
+        if top is not None:
+            if history:
+                raise InferError("a run that keeps its picks on the device does not score them")
+            n = ctx.B * (2 + 2 * top)
+            self.top = top
+            self.score_box = torch.empty(n, dtype=torch.int32, device=rt.device)
+            self.scores = Scores.packed(self.score_box, ctx.B, top)
+            self.score_ring = torch.empty((self.DEPTH, n), dtype=torch.int32).pin_memory()
 
     # ------------------------------------------------------------------ stepping
     def launch(self) -> None:
@@ -68,6 +80,9 @@ class DecodeRun:
         ctx.max_len = max(self.past) + self.launched + 1   # the positions moved on on the device
         logits = eng._forward(ctx)
         self.sampler.pick(logits, ctx.seq_slot, self.sampling, self.vocab_limit, out=self.box)
+        if self.scores is not None:
+            token_scores(logits, self.box, self.top, self.vocab_limit, self.scores)
+            self.score_ring[self.launched % self.DEPTH].copy_(self.score_box, non_blocking=True)
         K.advance_decode(ctx.tok_ids, ctx.tok_pos, self.box,
                          self.history[self.launched] if self.history is not None else None,
                          ctx.seq_past)
@@ -84,13 +99,23 @@ class DecodeRun:
         if self.n_read >= self.launched:
             raise InferError("no launched step is unread")
         got = self.engine.rt.take_mail(self.n_read % self.DEPTH, self.ctx.B)
-        if self.order is not None:
-            rows, got = got, [0] * len(got)
-            for j, i in enumerate(self.order):
-                got[i] = rows[j]
         self.d2h_bytes += 4 * (1 + self.ctx.B)
+        if self.scores is not None:                 # copied ahead of the picks
+            ring = self.score_ring[self.n_read % self.DEPTH]
+            self.last_scores = self._in_slot_order(
+                Scores.packed(ring, self.ctx.B, self.top).on_host())
+            self.d2h_bytes += 4 * ring.numel()
+        got = self._in_slot_order(got)
         self.n_read += 1
         self.picks.append(got)
+        return got
+
+    def _in_slot_order(self, rows: list) -> list:
+        if self.order is None:
+            return rows
+        got = list(rows)
+        for j, i in enumerate(self.order):
+            got[i] = rows[j]
         return got
 
     def picks_on_device(self) -> torch.Tensor:

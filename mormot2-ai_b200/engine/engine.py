@@ -25,6 +25,7 @@ from ..cache.storage import CacheStorage
 from ..config.registry import config_of_folder
 from ..csrc import build
 from ..errors import CacheError, InferError
+from ..sampling.scores import Scores, candidates, check_top, token_scores
 from ..weights.binding import bind_tensors
 from ..weights.safetensors_file import SafeTensorsFolder
 from .batch import StepBuffers, StepContext
@@ -41,10 +42,21 @@ DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16,
 @dataclass
 class Entry:
     """The next tokens of one sequence in a step: its slot, the tokens, and the places among
-    these tokens whose logits are wanted (None: the last one)."""
+    these tokens whose logits are wanted (None: the last one). ``given``, for ``Engine.score``: a
+    token for every wanted place, whose probability there is asked for (places None: one for each
+    of ``tokens``; both None: the tokens that follow, ``tokens[1:]`` at all places but the last)."""
     slot: int
     tokens: Sequence[int]
     want: Optional[Sequence[int]] = None
+    given: Optional[Sequence[int]] = None
+
+
+@dataclass
+class _Scoring:
+    """What a step gives instead of logits: scores of these tokens, one a wanted row."""
+    given: np.ndarray
+    top: int
+    vocab_limit: Optional[int]
 
 
 @dataclass
@@ -233,6 +245,40 @@ class Engine:
         step that fails between its passes leaves lengths and fixed-size state as it found
         them. The logits of a decode step lie in memory that the next decode step writes
         again: copy them if they are to outlive it."""
+        return self._step(entries, None)
+
+    def score(self, entries: Sequence[Entry], top: int = 0,
+              vocab_limit: Optional[int] = None) -> Scores:
+        """A step that says of given tokens how probable they were: appends each entry's tokens
+        to its sequence, as ``step`` does, and returns the scores of its ``given`` tokens at the
+        wanted places, in the order of the entries and of their ``want``: log probabilities,
+        entropy and the ``top`` (up to 32) most probable alternatives, among the ids below
+        ``vocab_limit``. The logits of many rows are never stored."""
+        top = check_top(top, candidates(self.vocab_size, vocab_limit))
+        below = candidates(self.vocab_size, vocab_limit)
+        placed, given = [], []
+        for e in entries:
+            g, want = e.given, e.want
+            if g is None:
+                if want is not None:
+                    raise InferError(f"slot {e.slot}: wanted places without the tokens to score there")
+                g = e.tokens[1:]
+                want = np.arange(len(g))
+            g = np.asarray(g, dtype=np.int64).reshape(-1)
+            if want is None:
+                want = np.arange(len(e.tokens))
+            if len(want) != g.size:
+                raise InferError(f"slot {e.slot}: {g.size} tokens to score at {len(want)} places")
+            bad = (g < 0) | (g >= below)
+            if bad.any():
+                raise InferError(f"slot {e.slot}: token {int(g[bad][0])} to score is outside the "
+                                 f"vocabulary of {below}")
+            placed.append(Entry(e.slot, e.tokens, want))
+            given.append(g)
+        given = np.concatenate(given) if given else np.zeros(0, dtype=np.int64)
+        return self._step(placed, _Scoring(given, top, vocab_limit))
+
+    def _step(self, entries: Sequence[Entry], scoring: Optional[_Scoring]):
         if not entries:
             raise InferError("a step without entries")
         if self.run is not None:
@@ -257,8 +303,14 @@ class Engine:
                 if bad.any():
                     raise InferError(f"slot {e.slot}: token {int(tokens[bad][0])} is outside "
                                      f"the vocabulary of {self.vocab_size}")
-            want = [len(tokens) - 1] if e.want is None else [int(w) for w in e.want]
-            if any(not 0 <= w < len(tokens) for w in want):
+            if isinstance(e.want, np.ndarray):
+                want = e.want if len(tokens) > 1 else e.want.tolist()
+                outside = any(want) if len(tokens) == 1 else ( 
+                    want.size and not 0 <= want.min() <= want.max() < len(tokens))
+            else:
+                want = [len(tokens) - 1] if e.want is None else [int(w) for w in e.want]
+                outside = any(not 0 <= w < len(tokens) for w in want)
+            if outside:
                 raise InferError(f"slot {e.slot}: wanted places {want} among {len(tokens)} tokens")
             past = self.book.length[e.slot]
             if past + len(tokens) > self.max_context:
@@ -278,11 +330,14 @@ class Engine:
             if sum(len(s[3]) for s in seqs) > self.max_step_tokens:
                 raise InferError(f"a pass of the step wants more than {self.max_step_tokens} "
                                  "rows of logits (max_step_tokens)")
-        new_pages = self.book.reserve([(s, p + len(t)) for s, p, t, _ in plan])
-        self.cache.map_pages(new_pages)
+        self._map([s for s, _, _, _ in plan], [p for _, p, _, _ in plan],
+                  [len(t) for _, _, t, _ in plan])
 
-        out = None
-        if n_want and len(passes) > 1:
+        out = given = None
+        if scoring is not None:
+            out = Scores.empty(n_want, scoring.top, self.rt.device)
+            given = torch.from_numpy(scoring.given.astype(np.int32)).to(self.rt.device)
+        elif n_want and len(passes) > 1:
             out = torch.empty((n_want, self.vocab_size), dtype=torch.float32, device=self.rt.device)
         self.last_h2d_bytes = 0
         self.last_passes = len(passes)
@@ -294,10 +349,12 @@ class Engine:
             for seqs, dest in passes:
                 # (``on_state`` is shown the rows as the entries come)
                 ctx = self.buffers.fill(seqs, len(seqs) >= self.sort_from and self.on_state is None)
-                self.last_h2d_bytes += 4 * (4 * ctx.T + 3 * ctx.B + 1 + ctx.n_want)
-                if ctx.entry_slots is not ctx.seq_slot:
-                    self.last_h2d_bytes += 4 * ctx.B
+                self.last_h2d_bytes += self.buffers.copied_bytes
                 self.last_slots = ctx.entry_slots
+                if scoring is not None:
+                    self._score_pass(ctx, scoring, given, dest, out)
+                    self.passes += 1
+                    continue
                 logits = self._forward(ctx)
                 self.passes += 1
                 if logits is not None:
@@ -317,6 +374,12 @@ class Engine:
             self.ids[slot].extend(tokens.tolist() if isinstance(tokens, np.ndarray) else tokens)
         return out
 
+    def _map(self, slots: List[int], past: List[int], new: List[int]) -> None:
+        """Reserves the pages of sequences that grow by ``new`` positions (all or nothing) and
+        writes them to the page tables."""
+        grown = self.book.grow([(s, p + n) for s, p, n in zip(slots, past, new)])
+        self.cache.map_grown(slots, past, new, grown)
+
     def timed_step(self, entries: Sequence[Entry]):
         """``step`` with its kernels run one by one and timed by class: returns the logits, the
         milliseconds of each class (products, attention, norms, rotary, embedding, ...) and
@@ -334,6 +397,30 @@ class Engine:
             self.use_graphs = graphs
         shares = timing.shares(e0, e1)
         return logits, shares, e0.elapsed_time(e1)
+
+    def _score_pass(self, ctx: StepContext, scoring: _Scoring, given: torch.Tensor,
+                    dest: List[int], out: Scores) -> None:
+        """One pass whose wanted rows are scored: rows ``dest`` of ``out``."""
+        whole = ctx.n_want == out.logprobs.shape[0]      # a pass of all rows brings them in order
+        places = None
+        if not whole and ctx.n_want:
+            places = torch.tensor(dest, dtype=torch.long, device=given.device)
+            given = given.index_select(0, places)
+        if self.use_graphs and ctx.decode and self.on_state is None:
+            logits = self._forward(ctx)                  # a captured pass gives logits
+            if logits is None:
+                return
+            got = token_scores(logits, given, scoring.top, scoring.vocab_limit,
+                               out if whole else None)
+        else:
+            got = self.model.forward(ctx, self.cache, self.on_state,
+                                     (given, scoring.top, scoring.vocab_limit))
+            if got is None:
+                return
+        if not whole:
+            out.put(places, got)
+        elif got is not out:
+            out.take(got)
 
     # ------------------------------------------------------------------ one pass
     def _forward(self, ctx: StepContext) -> Optional[torch.Tensor]:
@@ -382,14 +469,17 @@ class Engine:
     # ------------------------------------------------------------------ decoding on the device
     def decode_run(self, slots: Sequence[int], tokens: Sequence[int], steps: Sequence[int],
                    sampler, sampling, vocab_limit: Optional[int] = None,
-                   history: bool = False) -> DecodeRun:
+                   history: bool = False, top: Optional[int] = None) -> DecodeRun:
         """Opens a decode run (``engine/decode.py``): the sequences in ``slots`` are fed
         ``tokens`` in its first step and from then on what the sampler chose for them in the
         step before, in device memory. ``steps[i]``: the most steps sequence i takes part in;
         its pages up to there are reserved now (all or nothing), and the run goes no further
-        than the smallest of them. Until the run is finished no other step may be made."""
+        than the smallest of them. ``top``: every choice is scored too, with so many alternatives
+        (``DecodeRun.last_scores``). Until the run is finished no other step may be made."""
         if self.run is not None:
             raise InferError("a decode run is open already")
+        if top is not None:
+            check_top(top, candidates(self.vocab_size, vocab_limit))
         if (len(set(slots)) != len(slots) or len(tokens) != len(slots)
                 or len(steps) != len(slots) or not slots):
             raise InferError("a decode run: one token and one step count for each of "
@@ -411,17 +501,16 @@ class Engine:
                 raise CacheError(f"slot {slot}: its fixed-size state does not hold its "
                                  f"{past} tokens: truncate it to 0 or close it")
             seqs.append((slot, past, [int(t)], [0]))
-        self.cache.map_pages(self.book.reserve(
-            [(s, p + n) for (s, p, _, _), n in zip(seqs, steps)]))
+        self._map([s for s, _, _, _ in seqs], [p for _, p, _, _ in seqs], list(steps))
         # Inside the run the longest sequence comes first: the attention's CTAs start in the
         # order of the rows, and the long ones must not be the last to start. The order holds
         # for the whole run, since every sequence grows by one position a step.
         order = sorted(range(len(seqs)), key=lambda i: -seqs[i][1])
         ctx = self.buffers.fill([seqs[i] for i in order])
-        self.last_h2d_bytes = 4 * (4 * ctx.T + 3 * ctx.B + 1 + ctx.n_want)
+        self.last_h2d_bytes = self.buffers.copied_bytes
         self.last_slots, self.last_passes = ctx.seq_slot, 1
         self.run = DecodeRun(self, ctx, list(slots), [int(t) for t in tokens], min(steps),
-                             sampler, sampling, vocab_limit, history, order)
+                             sampler, sampling, vocab_limit, history, order, top)
         return self.run
 
     def decode_steps(self, slots: Sequence[int], tokens: Sequence[int], n_steps: int, sampler,
@@ -452,14 +541,13 @@ class Engine:
             # wanted rows come out in the order of the entries already
             return [(plan, list(range(sum(len(p[3]) for p in plan))))]
         # output rows in the order of the entries and of their want
-        row_of: List[Dict[int, List[int]]] = []
+        rows_of: List[Tuple[np.ndarray, np.ndarray]] = []     # wanted places in order, their output rows
         at = 0
-        for _, _, tokens, want in plan:
-            d: Dict[int, List[int]] = {}
-            for w in want:
-                d.setdefault(w, []).append(at)
-                at += 1
-            row_of.append(d)
+        for _, _, _, want in plan:
+            want = np.asarray(want, dtype=np.int64)
+            order = np.argsort(want, kind="stable")
+            rows_of.append((want[order], at + order))
+            at += len(want)
         done = [0] * len(plan)
         passes = []
         while any(done[i] < len(plan[i][2]) for i in range(len(plan))):
@@ -471,13 +559,10 @@ class Engine:
                     continue
                 n = min(left, self.prefill_chunk, budget)
                 lo, hi = done[i], done[i] + n
-                w_here, d_here = [], []
-                for w in sorted(w for w in row_of[i] if lo <= w < hi):
-                    for r in row_of[i][w]:
-                        w_here.append(w - lo)
-                        d_here.append(r)
-                seqs.append((slot, past + lo, tokens[lo:hi], w_here))
-                dest.extend(d_here)
+                places, rows = rows_of[i]
+                a, b = np.searchsorted(places, (lo, hi))
+                seqs.append((slot, past + lo, tokens[lo:hi], (places[a:b] - lo).tolist()))
+                dest.extend(rows[a:b].tolist())
                 done[i] = hi
                 budget -= n
             passes.append((seqs, dest))

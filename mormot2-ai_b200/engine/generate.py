@@ -39,6 +39,7 @@ class Request:
 class Outcome:
     tokens: List[int]
     stopped: bool      # ended on a stop token (else on its cap)
+    scores: Optional[list] = None     # a ``TokenScore`` a token, where they were asked for
 
 
 def checked(requests: Sequence[Request], limit: int) -> List[Request]:
@@ -94,29 +95,38 @@ AHEAD = 2      # steps launched before the oldest of them is read
 
 
 def generate(stepper, requests: Sequence[Request]) -> List[Outcome]:
-    """Runs every request to its end and returns the new tokens of each, in request order."""
+    """Runs every request to its end and returns the new tokens of each, in request order. A
+    stepper whose ``top`` is not None also leaves the scores of its last picks in ``last_scores``, and
+    so do its runs."""
+    scored = getattr(stepper, "top", None) is not None
     reqs = checked(requests, stepper.context_limit())
     results: List[Optional[Outcome]] = [None] * len(reqs)
     for batch in plan_batches(reqs, stepper.max_batch(), stepper.pools()):
         live: Dict[int, int] = {}          # request index -> slot
         new: Dict[int, List[int]] = {i: [] for i in batch}
+        said: Dict[int, list] = {i: [] for i in batch}
 
-        def take(i: int, token: int) -> bool:
+        def take(i: int, token: int, score=None) -> bool:
             """Books a pick of request i; True if it was its last."""
             new[i].append(token)
+            if score is not None:
+                said[i].append(score)
             stopped = token in reqs[i].stop
             if stopped or len(new[i]) >= reqs[i].max_new:
-                results[i] = Outcome(new[i], stopped)
+                results[i] = Outcome(new[i], stopped, said[i] if scored else None)
                 return True
             return False
+
+        def scores_of(source, n: int) -> list:
+            return source.last_scores if scored else [None] * n
 
         run = None
         try:
             for i in batch:
                 live[i] = stepper.open(reqs[i].seed)
             picks = stepper.prefill([(live[i], reqs[i].prompt) for i in batch])
-            for i, token in zip(list(batch), picks):
-                if take(i, int(token)):
+            for i, token, score in zip(list(batch), picks, scores_of(stepper, len(picks))):
+                if take(i, int(token), score):
                     stepper.close(live.pop(i))       # the slot is free for a later batch
             while live:
                 members = [i for i in batch if i in live]
@@ -131,19 +141,21 @@ def generate(stepper, requests: Sequence[Request]) -> List[Outcome]:
                         run.launch()
                         launched += 1
                     tokens = run.read()
+                    scores = scores_of(run, len(tokens))
                     n_read += 1
                     for m, i in enumerate(members):
                         kept[m] += 1
-                        done[m] = take(i, int(tokens[m]))
+                        done[m] = take(i, int(tokens[m]), scores[m])
                 while n_read < launched:
                     # launched before the host knew that a sequence had ended: these steps
                     # still count for the sequences that go on
                     tokens = run.read()
+                    scores = scores_of(run, len(tokens))
                     n_read += 1
                     for m, i in enumerate(members):
                         if not done[m]:
                             kept[m] += 1
-                            done[m] = take(i, int(tokens[m]))
+                            done[m] = take(i, int(tokens[m]), scores[m])
                 run.finish(kept)
                 run = None
                 for m, i in enumerate(members):
@@ -161,8 +173,12 @@ class EngineStepper:
     """The engine and the device sampler as the stepper of ``generate``."""
 
     def __init__(self, engine, sampling, vocab_limit: Optional[int] = None,
-                 max_batch: Optional[int] = None):
+                 max_batch: Optional[int] = None, top: Optional[int] = None):
+        """``top``: score every pick, with so many alternatives (None: picks alone)."""
         from ..sampling.device import DeviceSampler
+        from ..sampling.scores import candidates, check_top
+        self.top = None if top is None else check_top(top, candidates(engine.vocab_size, vocab_limit))
+        self.last_scores: list = []
         import torch
         self.engine, self.sampling, self.vocab_limit = engine, sampling, vocab_limit
         self._max_batch = min(max_batch or engine.max_slots, engine.max_slots)
@@ -203,6 +219,11 @@ class EngineStepper:
         box = rt.token_box(rows)
         tokens = self.sampler.pick(logits, ctx_slots, self.sampling, self.vocab_limit, out=box)
         self.h2d_bytes += self.engine.last_h2d_bytes
+        if self.top is not None:
+            from ..sampling.scores import token_scores
+            scores = token_scores(logits, tokens, self.top, self.vocab_limit)
+            self.last_scores = scores.on_host()
+            self.d2h_bytes += 4 * rows * (2 + 2 * self.top)
         if box is None:
             host = tokens.cpu()
             rt.check()
@@ -215,7 +236,7 @@ class EngineStepper:
         """A decode run over ``members = [(slot, last pick, steps it may still take)]``."""
         run = self.engine.decode_run([m[0] for m in members], [m[1] for m in members],
                                      [m[2] for m in members], self.sampler, self.sampling,
-                                     self.vocab_limit)
+                                     self.vocab_limit, top=self.top)
         self.h2d_bytes += self.engine.last_h2d_bytes
         return _CountedRun(run, self)
 
@@ -228,7 +249,12 @@ class _CountedRun:
         self.launch, self.finish, self.abandon = run.launch, run.finish, run.abandon
 
     def read(self) -> List[int]:
+        before = self.run.d2h_bytes
         got = self.run.read()
-        self.stepper.d2h_bytes += 4 * (1 + len(got))
+        self.stepper.d2h_bytes += self.run.d2h_bytes - before
         self.stepper.decode_steps += 1
         return got
+
+    @property
+    def last_scores(self) -> list:
+        return self.run.last_scores

@@ -117,9 +117,11 @@ class DecoderModel:
             part.bind(weights, rt)
 
     # ---------------------------------------------------------------- one pass
-    def forward(self, step, cache, on_state=None) -> Optional[torch.Tensor]:
+    def forward(self, step, cache, on_state=None, score=None):
         """``cache``: the ``CacheStorage``. ``on_state(name, x)``: called with the residual
-        after the embedding and after every entry of the order (for tests)."""
+        after the embedding and after every entry of the order (for tests). ``score``: ``(tokens,
+        top, vocab_limit)``; the head then scores these tokens, one a wanted row, instead of giving
+        the rows' logits (``Scores``)."""
         # the residual: [T, hidden], or [streams, T, hidden] for a model of several streams
         shape = (step.T, self.spec.hidden_size)
         if self.spec.streams:
@@ -165,4 +167,4 @@ class DecoderModel:
         if step.n_want == 0:
             return None
         h = self.final_norm.forward(x, rows=step.want_rows, n_rows=step.n_want)
-        return self.head.forward(h)
+        return self.head.forward(h) if score is None else self.head.score(h, *score)

@@ -59,6 +59,24 @@ def _sms() -> int:
     return _sms_of(torch._C._cuda_getDevice())
 
 
+class _NoChange:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_no_change = _NoChange()
+
+
+def on_device_of(t: torch.Tensor):
+    """A ``with`` block whose launches go to the device of ``t`` and its current stream."""
+    if not t.is_cuda:
+        raise KernelError("a kernel was given a tensor that is not on the GPU")
+    return _no_change if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
 def require_gpu() -> None:
     if not torch.cuda.is_available():
         raise KernelError("no CUDA device: this library computes on a B200 only (no CPU path)")
@@ -80,7 +98,8 @@ CLASS_OF = {"mb_gemm_tc": "products", "mb_gemm_simt": "products",
             "mb_attention_prefill_tc": "attention", "mb_rmsnorm": "norms",
             "mb_qk_norm_rope_store": "rotary", "mb_embed": "embedding", "mb_swiglu": "activation",
             "mb_argmax": "sampling", "mb_sample": "sampling", "mb_sample_filtered": "sampling",
-            "mb_advance_decode": "sampling", "mb_dynamic_tanh": "norms",
+            "mb_advance_decode": "sampling", "mb_token_scores": "scores",
+            "mb_step_index": "indexes", "mb_map_pages": "indexes", "mb_dynamic_tanh": "norms",
             "mb_gated_act": "activation", "mb_scale": "activation", "mb_add_bias": "activation",
             "mb_gemm_tc_gated": "products", "mb_latent_prep": "rotary",
             "mb_heads_gemm": "products", "mb_latent_attention": "attention",
@@ -1474,6 +1493,92 @@ def sample(logits: torch.Tensor, temperature: float, state_index: torch.Tensor,
     _call("sampling", "mb_sample", [_vp, _ll, _i, _i, _d, _vp, _vp, _vp, _vp],
           _ptr(logits), logits.stride(0), rows, V, float(temperature), _ptr(state_index),
           _ptr(states), _ptr(out), _stream())
+
+
+TOP_SCORES = 32          # alternatives of a row at most (MB_SCORES_TOP in csrc/scores.cuh)
+
+
+def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int, logprobs: torch.Tensor,
+                 entropy: torch.Tensor, top_ids: torch.Tensor, top_logprobs: torch.Tensor) -> None:
+    """Per row of ``logits`` [rows, V] (float32): the log probability of ``tokens[row]`` (int32; NaN
+    where that is no id below V), the entropy, and the ids and log probabilities of the ``top``
+    greatest logits, the lowest id first among equals. The outputs are contiguous."""
+    rows, V = logits.shape
+    assert logits.dtype == torch.float32 and (V == 1 or logits.stride(1) == 1)
+    assert tokens.dtype == torch.int32 and tokens.is_contiguous() and tokens.numel() == rows
+    assert logprobs.dtype == entropy.dtype == top_logprobs.dtype == torch.float32
+    assert top_ids.dtype == torch.int32
+    assert logprobs.numel() == entropy.numel() == rows
+    assert top_ids.numel() == top_logprobs.numel() == rows * top
+    for t in (logprobs, entropy, top_ids, top_logprobs):
+        _contig(t, "an output of the scores")
+    f, _ = _functions.get("mb_token_scores_scratch") or _function(
+        "scores", "mb_token_scores_scratch", [_i, _i, _i], _ll)
+    scratch = torch.empty(f(rows, V, top), dtype=torch.uint8, device=logits.device)
+    _call("scores", "mb_token_scores",
+          [_vp, _ll, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
+          _ptr(logits), logits.stride(0), rows, V, _ptr(tokens), top, _ptr(logprobs),
+          _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs), _ptr(scratch), scratch.numel(),
+          _stream(), launches=2)
+
+
+# ------------------------------------------------------------------------------ a step's arrays
+def _sequences(what: str, **lists) -> int:
+    """The length of int32 lists, which is the same for all of them, as is their device."""
+    first = next(iter(lists.values()))
+    n = first.numel()
+    for name, t in lists.items():
+        if (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.numel() != n
+                or t.device != first.device):
+            raise KernelError(f"{what}: {name} is {t.dtype} {tuple(t.shape)} on {t.device}, not a "
+                              f"contiguous int32 list of {n} on {first.device}")
+    return n
+
+
+def _same_device(what: str, first: torch.Tensor, *others: torch.Tensor) -> None:
+    for t in others:
+        if t.device != first.device:
+            raise KernelError(f"{what}: tensors on {first.device} and on {t.device}")
+
+
+def step_index(slots: torch.Tensor, past: torch.Tensor, new: torch.Tensor, seq_start: torch.Tensor,
+               tok_seq: torch.Tensor, tok_pos: torch.Tensor, tok_slot: torch.Tensor) -> None:
+    """The arrays of a step that packs the sequences one after another, ``new[b]`` tokens each
+    behind the ``past[b]`` that its slot holds (none where it is 0): ``seq_start`` [B + 1] their first
+    rows and the end; per token its sequence, position and slot. The token arrays may be longer than
+    the step (what lies behind it is left) or shorter (what does not fit is not written). All
+    int32, on the device; nothing is read on the host."""
+    B = _sequences("step_index", slots=slots, past=past, new=new)
+    if _sequences("step_index", seq_start=seq_start) != B + 1:
+        raise KernelError(f"step_index: seq_start holds {seq_start.numel()} rows, not {B} + 1")
+    T = _sequences("step_index", tok_seq=tok_seq, tok_pos=tok_pos, tok_slot=tok_slot)
+    _same_device("step_index", slots, seq_start, tok_seq)
+    with on_device_of(slots):
+        _call("step_index", "mb_step_index", [_vp, _vp, _vp, _i, _ll, _vp, _vp, _vp, _vp, _vp],
+              _ptr(slots), _ptr(past), _ptr(new), B, T, _ptr(seq_start), _ptr(tok_seq),
+              _ptr(tok_pos), _ptr(tok_slot), _stream())
+
+
+def map_pages(table: torch.Tensor, slots: torch.Tensor, past: torch.Tensor, new: torch.Tensor,
+              held: torch.Tensor, pages: torch.Tensor, ring_pages: int = 0) -> None:
+    """The pages that sequences grow into, written to their rows of ``table`` [slots, max_pages]:
+    row ``slots[b]`` holds ``held[b]`` pages and receives the next ones of ``pages`` up to what
+    ``past[b] + new[b]`` positions take (at most ``ring_pages``, where that is above 0), sequence
+    after sequence. Distinct slots. Entries outside the table are left, and so are those that ``pages``
+    is too short for. All int32, on the device; nothing is read on the host."""
+    B = _sequences("map_pages", slots=slots, past=past, new=new, held=held)
+    N = _sequences("map_pages", pages=pages)
+    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        raise KernelError(f"map_pages: the table is {table.dtype} {tuple(table.shape)}, not a "
+                          "contiguous int32 matrix")
+    if ring_pages < 0:
+        raise KernelError(f"map_pages: a ring of {ring_pages} pages")
+    _same_device("map_pages", slots, table, pages)
+    with on_device_of(slots):
+        _call("step_index", "mb_map_pages",
+              [_vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _vp],
+              _ptr(table), table.shape[0], table.shape[1], _ptr(slots), _ptr(past), _ptr(new),
+              _ptr(held), B, _ptr(pages), N, ring_pages, _stream())
 
 
 # ------------------------------------------------------------------------------ tensor cores

@@ -5,13 +5,18 @@ multiplies its float32 logits by that constant; one with ``softcap`` c turns the
 c tanh(logits / c))."""
 from __future__ import annotations
 
-from typing import Dict, List
+from typing import Dict, List, Optional
 
 import torch
 
 from .. import kernels as K
+from ..sampling.scores import Scores, check_score, token_scores
 from .base import EMBEDDINGS, ENTRIES, HEADS, Part, TensorNeed
 from .linear import Linear, Pending
+
+
+# Rows whose logits are stored at a time where they are scored through memory
+SCORE_BAND = 256
 
 
 class TokenEmbedding(Part):
@@ -64,6 +69,21 @@ class LmHead(Part):
         if self.softcap > 0:
             K.softcap_rows(logits, self.softcap)
         return logits
+
+    def libraries(self, rt):
+        return ["scores"]
+
+    def score(self, h: torch.Tensor, tokens: torch.Tensor, top: int = 0,
+              vocab_limit: Optional[int] = None) -> Scores:
+        """The scores of ``tokens`` (int32 [rows]) under the logits of ``h`` [rows, hidden], as
+        ``token_scores`` of ``forward(h)`` gives them, without the logits of all rows at once."""
+        check_score(h, tokens, top, self.hidden, self.vocab, vocab_limit)
+        rows = h.shape[0]
+        out = Scores.empty(rows, top, h.device)
+        for a in range(0, rows, SCORE_BAND):
+            b = min(rows, a + SCORE_BAND)
+            token_scores(self.forward(h[a:b]), tokens[a:b], top, vocab_limit, out.rows(a, b))
+        return out
 
 
 class PassInput(Part):

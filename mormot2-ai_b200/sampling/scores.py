@@ -1,0 +1,138 @@
+"""What a model says of given tokens: their log probabilities, the entropy of the row they were drawn
+from, and the most probable alternatives, on the device (``csrc/scores.cu``). The probabilities are
+the model's own, of the whole vocabulary: no temperature and no filter is in them. The reference
+returns chosen tokens only; scores are this library's own."""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import List, Optional, Tuple
+
+import torch
+
+from .. import kernels as K
+from ..errors import InferError
+
+
+@dataclass
+class TokenScore:
+    """The scores of one token on the host: its log probability, the entropy of what it was chosen
+    from, and the most probable ids with their log probabilities."""
+    logprob: float
+    entropy: float
+    alternatives: List[Tuple[int, float]]
+
+
+@dataclass
+class Scores:
+    """One entry a row: ``logprobs`` and ``entropy`` (natural logarithms, float32 [rows]); the ids
+    (int32) and log probabilities of the alternatives [rows, top], the most probable first and the
+    lowest id first among equals. A row with a NaN or a positive infinity among its logits, or with
+    nothing but negative infinities, has no distribution: its numbers are NaN (its ids are still in the
+    order of the logits, a NaN last)."""
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+    @classmethod
+    def empty(cls, rows: int, top: int, device) -> "Scores":
+        return cls(torch.empty(rows, dtype=torch.float32, device=device),
+                   torch.empty(rows, dtype=torch.float32, device=device),
+                   torch.empty((rows, top), dtype=torch.int32, device=device),
+                   torch.empty((rows, top), dtype=torch.float32, device=device))
+
+    @classmethod
+    def packed(cls, buffer: torch.Tensor, rows: int, top: int) -> "Scores":
+        """Scores that lie in an int32 ``buffer`` of ``rows * (2 + 2 * top)`` values one after
+        another, so that one copy brings them elsewhere."""
+        n = rows * top
+        ids = buffer[2 * rows:2 * rows + n].view(rows, top)
+        f = buffer.view(torch.float32)
+        return cls(f[:rows], f[rows:2 * rows], ids, f[2 * rows + n:2 * rows + 2 * n].view(rows, top))
+
+    def rows(self, a: int, b: int) -> "Scores":
+        """Rows a .. b - 1, in the same memory."""
+        return Scores(self.logprobs[a:b], self.entropy[a:b], self.top_ids[a:b],
+                      self.top_logprobs[a:b])
+
+    def put(self, places: torch.Tensor, rows: "Scores") -> None:
+        """``rows`` go to ``places`` (int64, on the device) of these."""
+        for mine, theirs in zip(self.tensors(), rows.tensors()):
+            mine.index_copy_(0, places, theirs)
+
+    def take(self, rows: "Scores") -> None:
+        """All of ``rows``, copied."""
+        for mine, theirs in zip(self.tensors(), rows.tensors()):
+            mine.copy_(theirs)
+
+    def on_host(self) -> List["TokenScore"]:
+        """One ``TokenScore`` a row (waits for the device)."""
+        lp, en, ids, alt = (t.tolist() for t in self.tensors())
+        return [TokenScore(a, b, list(zip(i, c))) for a, b, i, c in zip(lp, en, ids, alt)]
+
+    def tensors(self):
+        return self.logprobs, self.entropy, self.top_ids, self.top_logprobs
+
+
+def candidates(vocab: int, vocab_limit: Optional[int]) -> int:
+    """How many ids take part: all, or those below ``vocab_limit``."""
+    if vocab_limit is None:
+        return vocab
+    if vocab_limit < 1:
+        raise InferError(f"scores among the ids below {vocab_limit}")
+    return min(vocab, vocab_limit)
+
+
+def check_top(top: int, vocab: int) -> int:
+    if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= min(K.TOP_SCORES, vocab):
+        raise InferError(f"{top} alternatives: 0 to {min(K.TOP_SCORES, vocab)} can be had")
+    return top
+
+
+def check_tokens(tokens: torch.Tensor, rows: int, device) -> None:
+    if (tokens.dtype != torch.int32 or tokens.dim() != 1 or tokens.shape[0] != rows
+            or tokens.device != device):
+        raise InferError(f"scores of {rows} rows on {device}: tokens are {tokens.dtype} "
+                         f"{tuple(tokens.shape)} on {tokens.device}, not int32 [{rows}] there")
+
+
+def check_score(h: torch.Tensor, tokens: torch.Tensor, top: int, hidden: int, vocab: int,
+                vocab_limit: Optional[int]) -> int:
+    """Refuses what a head of ``vocab`` rows of ``hidden`` values cannot score; how many ids take
+    part."""
+    if h.dim() != 2 or h.shape[1] != hidden or (hidden > 1 and h.stride(1) != 1):
+        raise InferError(f"scores: the head's input is {tuple(h.shape)} with strides {h.stride()}, not "
+                         f"rows of {hidden} values")
+    vocab = candidates(vocab, vocab_limit)
+    check_top(top, vocab)
+    check_tokens(tokens, h.shape[0], h.device)
+    return vocab
+
+
+def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
+                 vocab_limit: Optional[int] = None, out: Optional[Scores] = None) -> Scores:
+    """The scores of ``tokens`` (int32 [rows]) under ``logits`` (float32 [rows, vocab], both on the
+    device; rows may lie apart). An id that is none of the vocabulary (-1 for "no token") scores NaN.
+    ``top``: alternatives, up to 32. ``vocab_limit``: only the ids below it take part. ``out``: to
+    write into, contiguous, as ``Scores.empty`` makes it. Runs on the current stream of the logits'
+    device and reads nothing back; what it needs besides is allocated for the call alone."""
+    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.shape[1] == 0:
+        raise InferError(f"scores: logits are {logits.dtype} {tuple(logits.shape)}, not float32 "
+                         "[rows, vocab]")
+    if logits.shape[1] > 1 and logits.stride(1) != 1:
+        raise InferError("scores: the logits of a row do not lie side by side")
+    rows, vocab = logits.shape[0], candidates(logits.shape[1], vocab_limit)
+    check_top(top, vocab)
+    check_tokens(tokens, rows, logits.device)
+    if vocab < logits.shape[1]:
+        logits = logits[:, :vocab]
+    if out is None:
+        out = Scores.empty(rows, top, logits.device)
+    elif out.top_ids.shape != (rows, top) or out.logprobs.device != logits.device:
+        raise InferError(f"scores of {rows} rows and {top} alternatives into {tuple(out.top_ids.shape)} "
+                         f"on {out.logprobs.device}")
+    if rows == 0:
+        return out
+    with K.on_device_of(logits):
+        K.token_scores(logits, tokens.contiguous(), top, *out.tensors())
+    return out

@@ -1,0 +1,287 @@
+"""Scores of given tokens from stored logits and from the rows before the head, against 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+from mormot2_ai_b200 import InferError, PartSpec, Runtime, token_scores
+from mormot2_ai_b200.parts import HEADS
+from mormot2_ai_b200.sampling import Scores
+from tests import score_oracle as oracle
+from tests.gpu_helpers import DEV
+
+pytestmark = pytest.mark.gpu
+
+LOWEST = float(np.finfo(np.float32).min)
+
+
+def logits_of(kind, rows, V, seed):
+    rng = np.random.default_rng(seed)
+    x = (rng.standard_normal((rows, V)) * 2.5).astype(np.float32)
+    if kind == "masked":
+        x[rng.random((rows, V)) < 0.97] = -np.inf
+    elif kind == "lowest":                       # masks of the type's lowest value
+        x[rng.random((rows, V)) < 0.9] = LOWEST
+        x[0] = LOWEST
+    elif kind == "ties":
+        x = np.round(x).astype(np.float32)
+        x[0] = 0.0
+        x[-1] = -0.0
+        x[-1, ::2] = 0.0
+    elif kind == "peaked":
+        x[np.arange(rows), rng.integers(0, V, rows)] += 40.0
+    elif kind == "one left":
+        keep = rng.integers(0, V, rows)
+        kept = x[np.arange(rows), keep].copy()
+        x[:] = -np.inf
+        x[np.arange(rows), keep] = kept
+    elif kind == "large":
+        x = (x * 1e36).astype(np.float32)
+    elif kind == "sorted":
+        x.sort(axis=1)
+        x[::2] = x[::2, ::-1]
+    elif kind == "broken":                       # rows without a distribution, between ordinary ones
+        x[0, V // 2] = np.nan
+        x[1 % rows, 0] = np.inf
+        x[2 % rows] = -np.inf
+        x[3 % rows] = np.nan
+        x[4 % rows, V - 1] = np.nan
+        x[4 % rows, 0] = np.inf
+    tokens = rng.integers(0, V, rows).astype(np.int32)
+    return x, tokens
+
+
+def on_device(x, pad=0, shift=0):
+    """x on the device with rows ``pad`` values apart, ``shift`` values behind an aligned address."""
+    rows, V = x.shape
+    buf = torch.full((rows * (V + pad) + shift,), 777.0, device=DEV)
+    view = buf[shift:].view(rows, V + pad)[:, :V]
+    view.copy_(torch.from_numpy(x))
+    return view
+
+
+KINDS = ["normal", "masked", "lowest", "ties", "peaked", "one left", "large", "sorted", "broken"]
+
+
+@pytest.mark.parametrize("rows,V,top,pad,shift", [
+    (1, 1, 0, 0, 0), (1, 1, 1, 0, 0), (3, 33, 32, 0, 0), (2, 509, 5, 3, 1), (5, 4096, 20, 0, 0),
+    (7, 8193, 1, 7, 2), (6, 40000, 32, 5, 3), (5, 151936, 20, 0, 0), (5, 151937, 7, 0, 1)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_token_scores(kind, rows, V, top, pad, shift):
+    x, tokens = logits_of(kind, rows, V, seed=rows * 1000 + V)
+    got = token_scores(on_device(x, pad, shift), torch.from_numpy(tokens).to(DEV), top)
+    oracle.check(got, x, tokens, top)
+
+
+def test_many_rows():
+    x, tokens = logits_of("normal", 70001, 40, seed=5)
+    got = token_scores(on_device(x), torch.from_numpy(tokens).to(DEV), 3)
+    lp, h, ids, alt = (t.cpu().numpy() for t in got.tensors())
+    y = x.astype(np.float64)
+    logp = y - y.max(1, keepdims=True)
+    logp -= np.log(np.exp(logp).sum(1, keepdims=True))
+    assert np.abs(lp - logp[np.arange(len(x)), tokens]).max() < 2e-5
+    assert np.array_equal(ids, np.argsort(-y, axis=1, kind="stable")[:, :3])
+    assert np.abs(alt - np.take_along_axis(logp, ids.astype(int), 1)).max() < 2e-5
+
+
+def test_places_beyond_32_bits():
+    """Rows whose distance passes 2^31 values."""
+    V, apart = 3000, (1 << 30) + 12
+    buf = torch.zeros(2 * apart + V, device=DEV)
+    x, tokens = logits_of("normal", 3, V, seed=9)
+    view = torch.as_strided(buf, (3, V), (apart, 1))
+    view.copy_(torch.from_numpy(x))
+    oracle.check(token_scores(view, torch.from_numpy(tokens).to(DEV), 4), x, tokens, 4)
+
+
+def test_ids_that_are_none():
+    x, _ = logits_of("normal", 5, 1000, seed=1)
+    tokens = torch.tensor([-1, 1000, 2 ** 31 - 1, -2 ** 31, 999], dtype=torch.int32, device=DEV)
+    got = token_scores(on_device(x), tokens, 2)
+    oracle.check(got, x, tokens.tolist(), 2)
+    assert torch.isnan(got.logprobs[:4]).all() and torch.isfinite(got.logprobs[4])
+
+
+def test_vocab_limit_and_out():
+    x, tokens = logits_of("normal", 4, 2000, seed=2)
+    tokens = tokens % 1500
+    out = Scores.empty(4, 6, DEV)
+    got = token_scores(on_device(x), torch.from_numpy(tokens).to(DEV), 6, 1500, out)
+    assert got is out
+    oracle.check(out, x[:, :1500], tokens, 6)
+    token_scores(on_device(x), torch.from_numpy(tokens).to(DEV), 6, 5000, out)
+    oracle.check(out, x, tokens, 6)
+    with pytest.raises(InferError):
+        token_scores(on_device(x), torch.from_numpy(tokens).to(DEV), 5, None, out)
+    packed = Scores.packed(torch.empty(4 * 14, dtype=torch.int32, device=DEV), 4, 6)
+    token_scores(on_device(x), torch.from_numpy(tokens).to(DEV), 6, None, packed)
+    for a, b in zip(packed.tensors(), out.tensors()):
+        assert torch.equal(a, b)
+
+
+def test_no_rows():
+    got = token_scores(torch.empty((0, 50), device=DEV), torch.empty(0, dtype=torch.int32, device=DEV), 3)
+    assert got.logprobs.shape == (0,) and got.top_ids.shape == (0, 3) and got.on_host() == []
+
+
+def test_the_same_again_on_streams_and_in_graphs():
+    """Equal bits from call to call, on a stream of its own, and from two graphs that are replayed
+    beside each other."""
+    x, tokens = logits_of("normal", 9, 60000, seed=3)
+    dx, dt = on_device(x), torch.from_numpy(tokens).to(DEV)
+    want = token_scores(dx, dt, 20)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = token_scores(dx, dt, 20)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(want.tensors(), got.tensors()):
+        assert torch.equal(a, b)
+    graphs, outs, ins = [], [], []
+    for k in range(2):
+        xk = dx.clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(token_scores(xk, dt, 20))
+        graphs.append(g)
+        ins.append(xk)
+    ins[1].copy_(dx.flip(0))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    other = token_scores(dx.flip(0).contiguous(), dt, 20)
+    for got, ref in ((outs[0], want), (outs[1], other)):
+        for a, b in zip(ref.tensors(), got.tensors()):
+            assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------- the head
+def make_head(weight, dtype, **more):
+    rt = Runtime(dtype, DEV)
+    head = HEADS.build(PartSpec("lm_head", {"name": "w", "tied": False, "vocab_size": weight.shape[0],
+                                            "hidden_size": weight.shape[1], **more}))
+    head.bind({"w": weight}, rt)
+    return head
+
+
+def grid(rng, shape, std, step):
+    """Whole multiples of ``step``: their products add up without a rounding in any order."""
+    return np.clip(np.round(rng.standard_normal(shape) * std / step), -255, 255) * step
+
+
+def head_case(rows, V, K, seed, dtype):
+    rng = np.random.default_rng(seed)
+    h = grid(rng, (rows, K), 1.0, 2.0 ** -5)
+    w = grid(rng, (V, K), 2.0 / np.sqrt(K), 2.0 ** -9)
+    tokens = rng.integers(0, V, rows).astype(np.int32)
+    dev = lambda a: torch.from_numpy(a).to(dtype).to(DEV)
+    return h, w, tokens, dev(h), dev(w), torch.from_numpy(tokens).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("rows,V,K,top", [
+    (1, 257, 64, 5), (1, 40000, 128, 32), (16, 1000, 96, 1), (17, 3001, 64, 0), (64, 5003, 192, 20),
+    (65, 2048, 72, 7), (128, 509, 256, 32), (129, 700, 64, 5), (255, 20000, 64, 20), (256, 256, 128, 3),
+    (257, 4099, 64, 32), (300, 33, 200, 32), (513, 30011, 64, 5), (1100, 5000, 100, 8)])
+def test_head_scores(dtype, rows, V, K, top):
+    h, w, tokens, dh, dw, dt = head_case(rows, V, K, rows + V, getattr(torch, dtype))
+    head = make_head(dw, getattr(torch, dtype))
+    got = head.score(dh, dt, top)
+    head.linear.rt.check()
+    oracle.check(got, h @ w.T, tokens, top)
+
+
+@pytest.mark.parametrize("rows", [5, 200, 300])
+@pytest.mark.parametrize("scale,cap", [(0.25, 0.0), (1.0, 3.0), (1.7, 5.0), (-1.0, 0.0), (0.0, 0.0)])
+def test_head_scale_and_cap(rows, scale, cap):
+    """The factor and the cap round: once a product, and for the cap by the division, tanhf (2 units,
+    its documented bound) and the product: 4 roundings of at most the cap's size."""
+    h, w, tokens, dh, dw, dt = head_case(rows, 3000, 128, 7, torch.bfloat16)
+    x = scale * (h @ w.T)
+    moved = 2.0 ** -24 * np.abs(x).max() * (scale not in (0.25, 1.0, -1.0, 0.0))
+    if cap:
+        moved = moved + 2.0 ** -24 * (np.abs(x).max() + 6 * cap)
+        x = cap * np.tanh(x / cap)
+    head = make_head(dw, torch.bfloat16, scale=scale, softcap=cap)
+    oracle.check(head.score(dh, dt, 9), x, tokens, 9, moved)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("rows", [3, 140, 270])
+def test_head_ordinary_values(dtype, rows):
+    """Values that do round: a logit may be off by a rounding of 2^-23 a product added up."""
+    rng = np.random.default_rng(rows)
+    t = getattr(torch, dtype)
+    dh = torch.from_numpy(rng.standard_normal((rows, 320))).to(t).to(DEV)
+    dw = torch.from_numpy(rng.standard_normal((2500, 320)) * 0.1).to(t).to(DEV)
+    tokens = rng.integers(0, 2500, rows).astype(np.int32)
+    h, w = dh.double().cpu().numpy(), dw.double().cpu().numpy()
+    moved = 320 * 2.0 ** -23 * (np.abs(h) @ np.abs(w).T).max(1)
+    got = make_head(dw, t).score(dh, torch.from_numpy(tokens).to(DEV), 12)
+    oracle.check(got, h @ w.T, tokens, 12, moved)
+
+
+@pytest.mark.parametrize("rows", [4, 200])
+def test_head_strides_limit_and_ties(rows):
+    """Rows that lie apart, ids below a limit, and a vocabulary whose every row stands twice."""
+    h, w, tokens, dh, dw, dt = head_case(rows, 2000, 64, 11, torch.bfloat16)
+    w[1000:] = w[:1000]
+    dw.copy_(torch.from_numpy(w))
+    wide = torch.zeros((rows, 64 + 24), dtype=torch.bfloat16, device=DEV)
+    wide[:, :64] = dh
+    dt = dt % 1501
+    head = make_head(dw, torch.bfloat16)
+    got = head.score(wide[:, :64], dt, 16, vocab_limit=1501)
+    oracle.check(got, (h @ w.T)[:, :1501], tokens % 1501, 16)
+    got = head.score(wide[:, :64], dt, 16, vocab_limit=10 ** 9)
+    oracle.check(got, h @ w.T, tokens % 1501, 16)
+    unaligned = torch.zeros((rows, 64 + 3), dtype=torch.bfloat16, device=DEV)
+    unaligned[:, 1:65] = dh
+    got = head.score(unaligned[:, 1:65], dt, 16)
+    oracle.check(got, h @ w.T, tokens % 1501, 16)
+
+
+@pytest.mark.parametrize("rows", [6, 300])
+def test_head_broken_rows(rows):
+    """A row with an infinity or a NaN has no distribution; its neighbours keep theirs."""
+    h, w, tokens, dh, dw, dt = head_case(rows, 3000, 64, 13, torch.bfloat16)
+    head = make_head(dw, torch.bfloat16)
+    want = head.score(dh, dt, 4)
+    dh[1, 3] = float("nan")
+    dh[rows - 1, 0] = float("inf")
+    got = head.score(dh, dt, 4)
+    bad = torch.zeros(rows, dtype=torch.bool, device=DEV)
+    bad[1] = bad[rows - 1] = True
+    assert torch.isnan(got.logprobs[bad]).all() and torch.isnan(got.entropy[bad]).all()
+    for a, b in zip(got.tensors(), want.tensors()):
+        assert torch.equal(a[~bad], b[~bad])
+
+
+def test_head_of_no_rows():
+    _, _, _, dh, dw, dt = head_case(1, 300, 64, 17, torch.bfloat16)
+    got = make_head(dw, torch.bfloat16).score(dh[:0], dt[:0], 4)
+    assert got.logprobs.shape == (0,) and got.top_ids.shape == (0, 4)
+
+
+def test_head_twice_and_in_graphs():
+    _, _, _, dh, dw, dt = head_case(300, 9000, 128, 19, torch.bfloat16)
+    head = make_head(dw, torch.bfloat16)
+    want = head.score(dh, dt, 20)
+    other = head.score(dh.flip(0).contiguous(), dt, 20)
+    graphs, outs = [], []
+    for x in (dh, dh.flip(0).contiguous()):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(head.score(x, dt, 20))
+        graphs.append((g, x))
+    for _ in range(5):
+        for g, _ in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for got, ref in zip(outs, (want, other)):
+        for a, b in zip(got.tensors(), ref.tensors()):
+            assert torch.equal(a, b)
