@@ -46,6 +46,7 @@ SOURCES = {
     "attention_simt": "attention_simt.cu",
     "sampling": "sampling.cu",
     "scores": "scores.cu",
+    "head_scores": "head_scores.cu",
     "step_index": "step_index.cu",
     "gemm_tc": "gemm_tc.cu",
     "attention_mma": "attention_mma.cu",
@@ -74,6 +75,7 @@ EXTRA_HEADERS = {"gemm_tc": ["tc_common.cuh"],
                  "attention_tc": ["attention_tc.cuh", "tc_common.cuh"],
                  "attention_diff_tc": ["attention_tc.cuh", "tc_common.cuh"],
                  "scores": ["scores.cuh"],
+                 "head_scores": ["scores.cuh", "tc_common.cuh"],
                  "latent": ["mma_common.cuh", "mma_tile.cuh"],
                  "moe": ["mma_common.cuh", "moe_act.cuh"],
                  "moe_tc": ["tc_common.cuh", "moe_act.cuh"],

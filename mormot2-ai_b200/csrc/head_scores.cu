@@ -1,0 +1,454 @@
+// Log probabilities of given tokens, entropy and the greatest alternatives straight from the rows
+// before the head: the product of rows [R, K] and the head [V, K] (bfloat16, float32 sums) on the
+// fifth-generation tensor cores, whose results never leave the chip. What a row has to keep of its V
+// logits is a mass (the maximum, S and T of scores.cuh) and `top` keys.
+//
+// A CTA pair (rank 0 issues tcgen05.mma.cta_group::2 for both) keeps 256 rows and walks a strip of
+// the vocabulary in tiles of up to 256 ids; 128 threads a CTA own a row each and fold a tile from
+// tensor memory into their row's mass and keys while the next tile is multiplied. At the strip's end
+// they leave both in memory; a block a row joins the strips (score_join_kernel in scores.cuh).
+//
+// The pairs that share a strip walk it side by side, so that its weights come from memory once and from
+// L2 for all row blocks but the first: a band of b row blocks takes floor(pairs / b) strips. Rows are
+// cut into bands such that few pairs idle (plan_bands).
+#include "scores.cuh"
+#include "tc_common.cuh"
+
+MB_DEFINE_LAST_ERROR
+
+#define HS_THREADS 192
+#define HS_BK 64
+#define HS_STAGES 5
+#define HS_HALF (128 * HS_BK * 2)            // one CTA's rows of an operand in a stage
+#define HS_BLOCKS 64                         // row blocks of 256 of a launch at most
+#define HS_LIST (MB_SCORES_TOP * 128 * 8)    // a key list for each of 128 rows
+#define HS_STAGED (4 * 32 * 128)             // 32 values of 32 rows for each epilogue warp
+#define HS_SMEM (1024 + HS_STAGES * 2 * HS_HALF + 256 + HS_LIST + HS_STAGED)
+
+// A band: `blocks` row blocks from `first` on, each in `strips` strips of `width` ids, tiles of `tile`
+struct HeadPlan {
+  int bands;
+  int first[HS_BLOCKS], blocks[HS_BLOCKS], strips[HS_BLOCKS], width[HS_BLOCKS], tile[HS_BLOCKS];
+  int part0[HS_BLOCKS];      // where a band's parts begin: [block][256 rows][strips]
+};
+
+// The tiles of a pair, the same for all of its warps
+struct HeadWalk {
+  const HeadPlan& plan;
+  int pair, limit, band, block, strip, n, end;
+  __device__ HeadWalk(const HeadPlan& p, int pair_, int limit_) : plan(p), pair(pair_), limit(limit_), band(-1) {
+    n = end = 0;
+  }
+  // the next strip of the pair; false when there is none
+  __device__ __forceinline__ bool next_strip() {
+    while (++band < plan.bands) {
+      const int b = plan.blocks[band];
+      if (pair >= b * plan.strips[band]) continue;
+      block = pair % b;
+      strip = pair / b;
+      n = strip * plan.width[band];
+      end = min(limit, n + plan.width[band]);
+      return true;
+    }
+    return false;
+  }
+  __device__ __forceinline__ int row0() const { return (plan.first[band] + block) * 256; }
+  __device__ __forceinline__ int cols() const { return min(plan.tile[band], end - n); }
+  __device__ __forceinline__ void step() { n += plan.tile[band]; }
+};
+
+// A row's greatest values so far: `top` keys in shared memory in no order (`list`: this row's first
+// one, 128 keys from one to the next), of which the least is known.
+struct TopList {
+  uint32_t list;
+  int top, worst;
+  TopKey least;
+  float bar;        // what a value has to pass: not (x <= bar); a NaN while the list has room
+
+  __device__ __forceinline__ void clear(uint32_t at, int top_) {
+    list = at;
+    top = top_;
+    worst = 0;
+    least = 0;
+    bar = __uint_as_float(0x7fc00000u);
+    for (int i = 0; i < top; ++i) put(i, 0);
+  }
+  __device__ __forceinline__ void put(int i, TopKey k) const {
+    asm volatile("st.shared.b64 [%0], %1;" ::"r"(list + i * 1024), "l"(k) : "memory");
+  }
+  __device__ __forceinline__ TopKey get(int i) const {
+    TopKey k;
+    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(k) : "r"(list + i * 1024) : "memory");
+    return k;
+  }
+  __device__ __forceinline__ void offer(TopKey k) {
+    if (k <= least) return;
+    put(worst, k);
+    TopKey m = ~(TopKey)0;
+    int at = 0;
+#pragma unroll 4
+    for (int i = 0; i < top; ++i) {
+      const TopKey c = get(i);
+      if (c < m) { m = c; at = i; }
+    }
+    least = m;
+    worst = at;
+    bar = m == 0 ? __uint_as_float(0x7fc00000u) : key_value(m);
+  }
+};
+
+// 32 columns of this thread's lane
+__device__ __forceinline__ void load32(uint32_t taddr, float* x) {
+  uint32_t a[16], b[16];
+  TMEM_LD16(a, 0);
+  TMEM_LD16(b, 16);
+  TMEM_HOLD16("tcgen05.wait::ld.sync.aligned;", a);
+  TMEM_HOLD16("", b);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    x[j] = __uint_as_float(a[j]);
+    x[16 + j] = __uint_as_float(b[j]);
+  }
+}
+// The head's factor and cap, as the kernels behind a stored product apply them
+__device__ __forceinline__ void shape32(float* x, float scale, float cap) {
+  if (scale != 1.f) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] *= scale;
+  }
+  if (cap > 0.f) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = cap * tanhf(x[j] / cap);
+  }
+}
+__device__ __forceinline__ float max32(const float* x) {
+  float m[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+  for (int j = 4; j < 32; ++j) m[j & 3] = fmaxf(m[j & 3], x[j]);
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+
+__global__ void __launch_bounds__(HS_THREADS, 1)
+head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ HeadPlan plan, int rows, int limit, int K, float scale,
+                   float cap, const int* __restrict__ tokens, int top, float* __restrict__ given,
+                   Mass* __restrict__ mass, TopKey* __restrict__ keys, int* __restrict__ error) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  const uint32_t sA = base, sB = base + HS_STAGES * HS_HALF;
+  const uint32_t bars = sB + HS_STAGES * HS_HALF;
+  const uint32_t full0 = bars, empty0 = bars + 8 * HS_STAGES;
+  const uint32_t acc_full0 = bars + 16 * HS_STAGES, acc_empty0 = acc_full0 + 16;
+  const uint32_t slot = acc_empty0 + 16;
+  const uint32_t lists = bars + 256, staged = lists + HS_LIST;
+  volatile uint32_t* slot_ptr = (volatile uint32_t*)(smem_raw + (slot - raw));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int nkb = (K + HS_BK - 1) / HS_BK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < HS_STAGES; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full0 + 8 * b, 1);
+      mbar_init(acc_empty0 + 8 * b, 8);      // the epilogue warps of both CTAs
+    }
+    mbar_fence_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) tmem_alloc_pair(slot, 512);
+  tc_fence_before_sync();
+  cluster_sync_all();
+  tc_fence_after_sync();
+  const uint32_t tmem = *slot_ptr;
+  mb_grid_wait();
+  mb_grid_launch_next();
+  HeadWalk walk(plan, blockIdx.x >> 1, limit);
+  if (warp == 0) {
+    if (elect_one()) {
+      int s = 0;
+      uint32_t ph = 0;
+      while (walk.next_strip()) {
+        const int m0 = walk.row0() + (int)rank * 128;
+        for (; walk.n < walk.end; walk.step()) {
+          // each CTA holds half of the tile's ids (whole boxes of 128 are copied)
+          const int n0 = walk.n + (int)rank * (((walk.cols() + 15) & ~15) >> 1);
+          for (int i = 0; i < nkb; ++i) {
+            mbar_wait(empty0 + 8 * s, ph ^ 1, error, 61);
+            if (rank == 0) mbar_expect_tx(full0 + 8 * s, 4 * HS_HALF);
+            const uint32_t full_lead = cluster_addr_of(full0 + 8 * s, 0);
+            tma_load_2d_pair(sA + s * HS_HALF, &tmA, i * HS_BK, m0, full_lead);
+            tma_load_2d_pair(sB + s * HS_HALF, &tmB, i * HS_BK, n0, full_lead);
+            if (++s == HS_STAGES) { s = 0; ph ^= 1; }
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      int s = 0, it = 0;
+      uint32_t ph = 0;
+      while (walk.next_strip()) {
+        for (; walk.n < walk.end; walk.step(), ++it) {
+          const uint32_t idesc = umma_idesc_bf16(256, (walk.cols() + 15) & ~15);
+          const int b = it & 1;
+          mbar_wait(acc_empty0 + 8 * b, ((it >> 1) & 1) ^ 1, error, 62);
+          tc_fence_after_sync();
+          for (int i = 0; i < nkb; ++i) {
+            mbar_wait(full0 + 8 * s, ph, error, 63);
+            tc_fence_after_sync();
+            const uint64_t da = umma_desc_k128(sA + s * HS_HALF);
+            const uint64_t db = umma_desc_k128(sB + s * HS_HALF);
+#pragma unroll
+            for (int k = 0; k < HS_BK / 16; ++k)
+              umma_bf16_pair(tmem + b * 256, da + 2 * k, db + 2 * k, idesc, (i | k) != 0);
+            umma_commit_pair(empty0 + 8 * s, 3);
+            if (++s == HS_STAGES) { s = 0; ph ^= 1; }
+          }
+          umma_commit_pair(acc_full0 + 8 * b, 3);
+        }
+      }
+    }
+  } else {
+    const int q = warp & 3;
+    const int lane_row = q * 32 + lane;
+    const uint32_t mine = staged + (uint32_t)q * 4096 + lane * 4;
+    const bool shaped = scale != 1.f || cap > 0.f;
+    int it = 0;
+    while (walk.next_strip()) {
+      const int in_block = (int)rank * 128 + lane_row, row = walk.row0() + in_block;
+      const int token = row < rows ? tokens[row] : -1;
+      float m = -INFINITY, s = 0.f, t = 0.f;     // the row's mass
+      TopList list;
+      list.clear(lists + lane_row * 8, top);
+      for (; walk.n < walk.end; walk.step(), ++it) {
+        const int b = it & 1, cols = walk.cols();
+        mbar_wait(acc_full0 + 8 * b, (it >> 1) & 1, error, 64);
+        tc_fence_after_sync();
+        float tile_s = 0.f, tile_t = 0.f;        // the tile's part, over the same maximum
+#pragma unroll 1
+        for (int c = 0; c < cols; c += 32) {
+          float x[32];
+          load32(tmem + b * 256 + ((uint32_t)(q * 32) << 16) + c, x);
+          const int n = min(32, cols - c), id0 = walk.n + c;
+          if (shaped) shape32(x, scale, cap);
+          if (n < 32) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j >= n) x[j] = -INFINITY;
+          }
+          const float most = max32(x);
+          if (most > m) {
+            const Mass row_part = mass_over({m, s, t}, most), tile_part = mass_over({m, tile_s, tile_t}, most);
+            m = most;
+            s = row_part.s, t = row_part.t;
+            tile_s = tile_part.s, tile_t = tile_part.t;
+          }
+          const float at = m == -INFINITY ? 0.f : m;
+          float ps[4] = {0.f, 0.f, 0.f, 0.f}, pt[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) mass_add(x[j], at, ps[j & 3], pt[j & 3]);
+          tile_s += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+          tile_t += (pt[0] + pt[1]) + (pt[2] + pt[3]);
+          const unsigned off = (unsigned)token - (unsigned)id0;
+          if (__any_sync(0xffffffffu, off < (unsigned)n)) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (off == (unsigned)j && j < n) given[row] = x[j];
+          }
+          if (top > 0 && __any_sync(0xffffffffu, !(most <= list.bar))) {
+            // Which values pass is a bit each; a lane takes its own one after another. They are read
+            // again from shared memory, where a register could not be named by a number.
+            unsigned pass = 0;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + j * 128), "f"(x[j]) : "memory");
+              if (!(x[j] <= list.bar)) pass |= 1u << j;
+            }
+            if (n < 32) pass &= (1u << n) - 1;
+            while (pass) {
+              const int j = __ffs(pass) - 1;
+              pass &= pass - 1;
+              float y;
+              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(mine + j * 128) : "memory");
+              list.offer(key_of(y, id0 + j));
+            }
+            __syncwarp();
+          }
+        }
+        s += tile_s;
+        t += tile_t;
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if (rank == 0) mbar_arrive(acc_empty0 + 8 * b);
+          else mbar_arrive_cluster(cluster_addr_of(acc_empty0 + 8 * b, 0));
+        }
+      }
+      if (row < rows) {
+        const int strips = plan.strips[walk.band];
+        const size_t part = plan.part0[walk.band] + ((size_t)walk.block * 256 + in_block) * strips + walk.strip;
+        mass[part] = {m, s, t};
+        for (int i = 0; i < top; ++i) keys[part * top + i] = list.get(i);
+      }
+    }
+  }
+  // neither CTA leaves while the other may still read its shared memory or signal its barriers
+  tc_fence_before_sync();
+  cluster_sync_all();
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+}
+
+// A block a row joins its strips.
+__global__ void __launch_bounds__(128)
+head_join_kernel(const __grid_constant__ HeadPlan plan, const Mass* __restrict__ mass,
+                 const TopKey* __restrict__ keys, int top, const float* __restrict__ given, int limit,
+                 const int* __restrict__ tokens, ScoreOut out) {
+  mb_grid_wait();
+  mb_grid_launch_next();
+  const int row = blockIdx.x;
+  int band = 0, block = row >> 8;
+  while (band + 1 < plan.bands && block >= plan.first[band + 1]) ++band;
+  block -= plan.first[band];
+  const int strips = plan.strips[band];
+  const size_t part = plan.part0[band] + ((size_t)block * 256 + (row & 255)) * strips;
+  const int token = tokens[row];
+  const bool ok = token >= 0 && token < limit;
+  join_parts(mass + part, keys + part * top, strips, top, ok ? given[row] : __uint_as_float(0x7fc00000u),
+             row, out);
+}
+
+static cudaError_t allow_smem() {
+  static unsigned long long done = 0;
+  return mb_allow_smem((const void*)head_scores_kernel, HS_SMEM, &done);
+}
+
+// How many CTA pairs the device runs at once (0: the kernel cannot run here)
+static int head_pairs(int sms) {
+  static int pairs = -1;
+  if (pairs >= 0) return pairs;
+  if (allow_smem() != cudaSuccess) {
+    cudaGetLastError();
+    return pairs = 0;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * sms);
+  cfg.blockDim = dim3(HS_THREADS);
+  cfg.dynamicSmemBytes = HS_SMEM;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, head_scores_kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  return pairs = n > sms / 2 ? sms / 2 : n;
+}
+
+// Ids of a strip where `blocks` row blocks share the pairs, a multiple of 16
+static int strip_width(int blocks, int pairs, int limit) {
+  const int strips = pairs / blocks;
+  return ((limit + strips - 1) / strips + 15) & ~15;
+}
+
+// Cuts `blocks` row blocks into bands of at most `pairs` blocks such that the strips' widths add up
+// to the least: the time of a band is that of its widest strip, and a strip's start and end.
+static void plan_bands(HeadPlan& plan, int blocks, int pairs, int limit) {
+  int best[HS_BLOCKS + 1], take[HS_BLOCKS + 1];
+  best[0] = 0;
+  for (int n = 1; n <= blocks; ++n) {
+    best[n] = 0x7fffffff;
+    for (int b = 1; b <= n && b <= pairs; ++b) {
+      const int cost = best[n - b] + strip_width(b, pairs, limit) + 64;
+      if (cost < best[n]) best[n] = cost, take[n] = b;
+    }
+  }
+  plan.bands = 0;
+  int first = 0, part = 0;
+  for (int n = blocks; n > 0; n -= take[n]) {
+    const int i = plan.bands++, b = take[n], width = strip_width(b, pairs, limit);
+    plan.first[i] = first;
+    plan.blocks[i] = b;
+    plan.width[i] = width;
+    plan.strips[i] = (limit + width - 1) / width;
+    const int tiles = (width + 255) / 256;
+    plan.tile[i] = ((width + tiles - 1) / tiles + 15) & ~15;
+    plan.part0[i] = part;
+    first += b;
+    part += b * 256 * plan.strips[i];
+  }
+}
+static int parts_of(const HeadPlan& plan) {
+  const int i = plan.bands - 1;
+  return plan.part0[i] + plan.blocks[i] * 256 * plan.strips[i];
+}
+
+// Whether mb_head_scores takes operands of these sizes and alignments on this device.
+MB_EXPORT int mb_head_scores_supported(const void* A, int lda, const void* W, int K, int sms) {
+  return K > 0 && K % 8 == 0 && lda % 8 == 0 && ((uintptr_t)A & 15) == 0 && ((uintptr_t)W & 15) == 0 &&
+         head_pairs(sms) > 0;
+}
+
+// bytes of scratch that mb_head_scores needs
+MB_EXPORT long long mb_head_scores_scratch(int rows, int limit, int top, int sms) {
+  const int pairs = head_pairs(sms);
+  if (pairs <= 0 || rows <= 0 || limit <= 0) return 0;
+  HeadPlan plan;
+  const int most = HS_BLOCKS * 256;
+  plan_bands(plan, ((rows < most ? rows : most) + 255) / 256, pairs, limit);
+  return (long long)parts_of(plan) * (12 + 8 * top) + 4ll * (rows < most ? rows : most) + 16;
+}
+
+// For rows A [rows, K] (bfloat16, `lda` values from row to row) and a head W [V, K]: the scores of
+// tokens[r] under the logits x = scale A W^T, or cap tanh(x / cap) where cap > 0, of the ids below
+// `limit` <= V. Outputs as mb_token_scores. scratch: mb_head_scores_scratch bytes, 16-byte aligned.
+MB_EXPORT int mb_head_scores(const void* A, int lda, const void* W, int rows, int limit, int K,
+                             float scale, float cap, const int* tokens, int top, float* logprobs,
+                             float* entropy, int* top_ids, float* top_logprobs, void* scratch,
+                             long long scratch_bytes, int* error, int sms, void* stream) {
+  if (rows <= 0) return 0;
+  if (limit <= 0 || top < 0 || top > MB_SCORES_TOP || top > limit)
+    MB_FAIL("mb_head_scores: %d alternatives of a vocabulary of %d", top, limit);
+  if (!mb_head_scores_supported(A, lda, W, K, sms))
+    MB_FAIL("mb_head_scores: rows of %d values, %d apart, are not taken", K, lda);
+  if (scratch_bytes < mb_head_scores_scratch(rows, limit, top, sms))
+    MB_FAIL("mb_head_scores: %lld bytes of scratch", scratch_bytes);
+  const int pairs = head_pairs(sms);
+  if (cudaError_t e = allow_smem()) MB_FAIL("mb_head_scores: %s", cudaGetErrorString(e));
+  cudaStream_t s = (cudaStream_t)stream;
+  CUtensorMap tmB;
+  if (!mb_make_map_bf16(&tmB, W, limit, K, K, 128, "mb_head_scores weight")) return -1;
+  for (int r0 = 0; r0 < rows; r0 += HS_BLOCKS * 256) {
+    const int n = rows - r0 < HS_BLOCKS * 256 ? rows - r0 : HS_BLOCKS * 256;
+    const __nv_bfloat16* a = (const __nv_bfloat16*)A + (size_t)r0 * lda;
+    HeadPlan plan = {};
+    plan_bands(plan, (n + 255) / 256, pairs, limit);
+    CUtensorMap tmA;
+    if (!mb_make_map_bf16(&tmA, a, n, K, lda, 128, "mb_head_scores input")) return -1;
+    const size_t parts = parts_of(plan);
+    TopKey* keys = (TopKey*)scratch;
+    Mass* mass = (Mass*)(keys + parts * top);
+    float* given = (float*)(mass + parts);
+    int used = 0;
+    for (int i = 0; i < plan.bands; ++i)
+      if (plan.blocks[i] * plan.strips[i] > used) used = plan.blocks[i] * plan.strips[i];
+    cudaError_t e = mb_launch_clusters(head_scores_kernel, dim3(2 * used), dim3(HS_THREADS), HS_SMEM, s,
+                                       2, tmA, tmB, plan, n, limit, K, scale, cap, tokens + r0, top,
+                                       given, mass, keys, error);
+    if (e != cudaSuccess) MB_FAIL("mb_head_scores: %s", cudaGetErrorString(e));
+    const ScoreOut out = {logprobs + r0, entropy + r0, top_ids + (size_t)r0 * top,
+                          top_logprobs + (size_t)r0 * top};
+    mb_launch(head_join_kernel, dim3(n), dim3(128), 0, s, plan, mass, keys, top, given, limit,
+              tokens + r0, out);
+  }
+  MB_CHECK_LAUNCH("mb_head_scores");
+}

@@ -8,27 +8,6 @@ MB_DEFINE_LAST_ERROR
 #define SCORE_THREADS 256
 #define SCORE_CHUNK 8192
 
-__device__ TopKey block_key_max(TopKey k, TopKey* sh) {
-  k = key_max_warp(k);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  __syncthreads();
-  if (lane == 0) sh[warp] = k;
-  __syncthreads();
-  k = sh[0];
-  for (int w = 1; w < warps; ++w)
-    if (sh[w] > k) k = sh[w];
-  return k;
-}
-__device__ Mass block_mass(Mass v, Mass* sh) {
-  v = mass_warp(v);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  if (lane == 0) sh[warp] = v;
-  __syncthreads();
-  v = sh[0];
-  for (int w = 1; w < warps; ++w) v = mass_join(v, sh[w]);
-  return v;
-}
-
 __global__ void __launch_bounds__(SCORE_THREADS)
 score_chunks_kernel(const float* __restrict__ logits, size_t stride, int V, int chunk, int top,
                     Mass* __restrict__ mass, TopKey* __restrict__ keys) {
@@ -60,39 +39,14 @@ score_chunks_kernel(const float* __restrict__ logits, size_t stride, int V, int 
 __global__ void __launch_bounds__(128)
 score_join_kernel(const Mass* __restrict__ mass, const TopKey* __restrict__ keys, int parts, int top,
                   const float* __restrict__ logits, size_t stride, int V,
-                  const int* __restrict__ tokens, float* __restrict__ logprobs,
-                  float* __restrict__ entropy, int* __restrict__ top_ids,
-                  float* __restrict__ top_logprobs) {
+                  const int* __restrict__ tokens, ScoreOut out) {
   mb_grid_wait();
   mb_grid_launch_next();
-  __shared__ Mass sh_mass[4];
-  __shared__ TopKey sh_key[4];
-  const int row = blockIdx.x;
-  Mass v = mass_none();
-  for (int p = threadIdx.x; p < parts; p += 128) v = mass_join(v, mass[(size_t)row * parts + p]);
-  v = block_mass(v, sh_mass);
-  const float ln_s = logf(v.s);
-  if (threadIdx.x == 0) {
-    const int t = tokens[row];
-    const bool ok = t >= 0 && t < V;
-    logprobs[row] = ok ? logits[(size_t)row * stride + t] - v.m - ln_s : __uint_as_float(0x7fc00000u);
-    const float h = ln_s - v.t / v.s;
-    entropy[row] = h < 0.f ? 0.f : h;
-  }
-  const TopKey* mine = keys + (size_t)row * parts * top;
-  TopKey last = ~(TopKey)0;
-  for (int j = 0; j < top; ++j) {
-    TopKey best = 0;
-    for (int i = threadIdx.x; i < parts * top; i += 128) {
-      const TopKey k = mine[i];
-      if (k < last && k > best) best = k;
-    }
-    last = block_key_max(best, sh_key);
-    if (threadIdx.x == 0) {
-      top_ids[(size_t)row * top + j] = key_id(last);
-      top_logprobs[(size_t)row * top + j] = key_value(last) - v.m - ln_s;
-    }
-  }
+  const int row = blockIdx.x, t = tokens[row];
+  const bool ok = t >= 0 && t < V;
+  const size_t part = (size_t)row * parts;
+  join_parts(mass + part, keys + part * top, parts, top,
+             ok ? logits[(size_t)row * stride + t] : __uint_as_float(0x7fc00000u), row, out);
 }
 
 static int chunks_of(int V) { return (V + SCORE_CHUNK - 1) / SCORE_CHUNK; }
@@ -121,6 +75,6 @@ MB_EXPORT int mb_token_scores(const float* logits, long long stride, int rows, i
   mb_launch(score_chunks_kernel, dim3(rows, parts), dim3(SCORE_THREADS), 0, s, logits, (size_t)stride,
             V, SCORE_CHUNK, top, mass, keys);
   mb_launch(score_join_kernel, dim3(rows), dim3(128), 0, s, mass, keys, parts, top, logits,
-            (size_t)stride, V, tokens, logprobs, entropy, top_ids, top_logprobs);
+            (size_t)stride, V, tokens, ScoreOut{logprobs, entropy, top_ids, top_logprobs});
   MB_CHECK_LAUNCH("mb_token_scores");
 }

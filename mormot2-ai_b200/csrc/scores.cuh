@@ -71,3 +71,60 @@ __device__ __forceinline__ TopKey key_max_warp(TopKey k) {
   }
   return k;
 }
+
+__device__ TopKey block_key_max(TopKey k, TopKey* sh) {
+  k = key_max_warp(k);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  __syncthreads();
+  if (lane == 0) sh[warp] = k;
+  __syncthreads();
+  k = sh[0];
+  for (int w = 1; w < warps; ++w)
+    if (sh[w] > k) k = sh[w];
+  return k;
+}
+__device__ Mass block_mass(Mass v, Mass* sh) {
+  v = mass_warp(v);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  if (lane == 0) sh[warp] = v;
+  __syncthreads();
+  v = sh[0];
+  for (int w = 1; w < warps; ++w) v = mass_join(v, sh[w]);
+  return v;
+}
+
+struct ScoreOut {
+  float *logprobs, *entropy;
+  int* top_ids;
+  float* top_logprobs;
+};
+
+// A block of 128 threads joins the parts of a row: their masses and, in any order, their keys.
+// `given`: the given token's logit, a NaN where there is none.
+__device__ void join_parts(const Mass* mass, const TopKey* keys, int parts, int top, float given, int row,
+                           const ScoreOut& out) {
+  __shared__ Mass sh_mass[4];
+  __shared__ TopKey sh_key[4];
+  Mass v = mass_none();
+  for (int p = threadIdx.x; p < parts; p += 128) v = mass_join(v, mass[p]);
+  v = block_mass(v, sh_mass);
+  const float ln_s = logf(v.s);
+  if (threadIdx.x == 0) {
+    out.logprobs[row] = given - v.m - ln_s;
+    const float h = ln_s - v.t / v.s;
+    out.entropy[row] = h < 0.f ? 0.f : h;
+  }
+  TopKey last = ~(TopKey)0;
+  for (int j = 0; j < top; ++j) {
+    TopKey best = 0;
+    for (int i = threadIdx.x; i < parts * top; i += 128) {
+      const TopKey k = keys[i];
+      if (k < last && k > best) best = k;
+    }
+    last = block_key_max(best, sh_key);
+    if (threadIdx.x == 0) {
+      out.top_ids[(size_t)row * top + j] = key_id(last);
+      out.top_logprobs[(size_t)row * top + j] = key_value(last) - v.m - ln_s;
+    }
+  }
+}

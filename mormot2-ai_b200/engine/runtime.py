@@ -82,7 +82,7 @@ class Runtime:
             raise KernelError(f"a kernel gave up a wait (code {code}: 1 load, 2 MMA, 3 epilogue, "
                               "6 accumulator; 4-5, 9-18 attention, 11-13 and 16 a product of CTA "
                               "pairs too; 41-48 float32 products in parts; 51-59 float32 attention "
-                              "in parts); its result is not valid")
+                              "in parts; 61-64 scores of a head's rows); its result is not valid")
 
     def token_box(self, rows: int) -> Optional[torch.Tensor]:
         """Where a sampler may leave ``rows`` chosen tokens for ``read_tokens`` (None: too many)."""

@@ -99,6 +99,7 @@ CLASS_OF = {"mb_gemm_tc": "products", "mb_gemm_simt": "products",
             "mb_qk_norm_rope_store": "rotary", "mb_embed": "embedding", "mb_swiglu": "activation",
             "mb_argmax": "sampling", "mb_sample": "sampling", "mb_sample_filtered": "sampling",
             "mb_advance_decode": "sampling", "mb_token_scores": "scores",
+            "mb_head_scores": "products",
             "mb_step_index": "indexes", "mb_map_pages": "indexes", "mb_dynamic_tanh": "norms",
             "mb_gated_act": "activation", "mb_scale": "activation", "mb_add_bias": "activation",
             "mb_gemm_tc_gated": "products", "mb_latent_prep": "rotary",
@@ -1520,6 +1521,39 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int, logprobs:
           _ptr(logits), logits.stride(0), rows, V, _ptr(tokens), top, _ptr(logprobs),
           _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs), _ptr(scratch), scratch.numel(),
           _stream(), launches=2)
+
+
+def head_scores_supported(h: torch.Tensor, w: torch.Tensor) -> bool:
+    """Whether ``head_scores`` takes these rows and this head."""
+    if h.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
+        return False
+    f, _ = _functions.get("mb_head_scores_supported") or _function(
+        "head_scores", "mb_head_scores_supported", [_vp, _i, _vp, _i, _i])
+    return bool(f(_ptr(h), h.stride(0), _ptr(w), w.shape[1], _sms()))
+
+
+def head_scores(h: torch.Tensor, w: torch.Tensor, limit: int, scale: float, cap: float,
+                tokens: torch.Tensor, top: int, logprobs: torch.Tensor, entropy: torch.Tensor,
+                top_ids: torch.Tensor, top_logprobs: torch.Tensor, error: torch.Tensor) -> None:
+    """``token_scores`` of the logits scale * h · wᵀ (of the first ``limit`` rows of ``w``; with ``cap``
+    > 0: cap tanh(x / cap)) for bfloat16 h [rows, K] and w [V, K], without storing them."""
+    rows, Kd = h.shape
+    assert w.shape[1] == Kd and h.stride(1) == 1 and 0 < limit <= w.shape[0]
+    assert tokens.dtype == torch.int32 and tokens.is_contiguous() and tokens.numel() == rows
+    assert logprobs.dtype == entropy.dtype == top_logprobs.dtype == torch.float32
+    assert top_ids.dtype == torch.int32 and logprobs.numel() == entropy.numel() == rows
+    assert top_ids.numel() == top_logprobs.numel() == rows * top
+    _contig(w, "the weight")
+    for t in (logprobs, entropy, top_ids, top_logprobs):
+        _contig(t, "an output of the scores")
+    f, _ = _functions.get("mb_head_scores_scratch") or _function(
+        "head_scores", "mb_head_scores_scratch", [_i, _i, _i, _i], _ll)
+    scratch = torch.empty(f(rows, limit, top, _sms()), dtype=torch.uint8, device=h.device)
+    _call("head_scores", "mb_head_scores",
+          [_vp, _i, _vp, _i, _i, _i, _f, _f, _vp, _i, _vp, _vp, _vp, _vp, _vp, _ll, _vp, _i, _vp],
+          _ptr(h), h.stride(0), _ptr(w), rows, limit, Kd, float(scale), float(cap), _ptr(tokens),
+          top, _ptr(logprobs), _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs), _ptr(scratch),
+          scratch.numel(), _ptr(error), _sms(), _stream(), launches=2 * -(-rows // 16384))
 
 
 # ------------------------------------------------------------------------------ a step's arrays

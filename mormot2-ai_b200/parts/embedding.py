@@ -15,6 +15,8 @@ from .base import EMBEDDINGS, ENTRIES, HEADS, Part, TensorNeed
 from .linear import Linear, Pending
 
 
+# bfloat16 rows up to which logits are stored and scored from there
+SCORE_STORED = 64
 # Rows whose logits are stored at a time where they are scored through memory
 SCORE_BAND = 256
 
@@ -71,18 +73,28 @@ class LmHead(Part):
         return logits
 
     def libraries(self, rt):
-        return ["scores"]
+        return ["scores", "head_scores"] if rt.fast_kernels else ["scores"]
 
     def score(self, h: torch.Tensor, tokens: torch.Tensor, top: int = 0,
               vocab_limit: Optional[int] = None) -> Scores:
         """The scores of ``tokens`` (int32 [rows]) under the logits of ``h`` [rows, hidden], as
-        ``token_scores`` of ``forward(h)`` gives them, without the logits of all rows at once."""
-        check_score(h, tokens, top, self.hidden, self.vocab, vocab_limit)
+        ``token_scores`` of ``forward(h)`` gives them. Of more than a few bfloat16 rows the logits are
+        never stored (``csrc/head_scores.cu``); others go through memory, a band of rows at a time."""
+        limit = check_score(h, tokens, top, self.hidden, self.vocab, vocab_limit)
         rows = h.shape[0]
         out = Scores.empty(rows, top, h.device)
-        for a in range(0, rows, SCORE_BAND):
-            b = min(rows, a + SCORE_BAND)
-            token_scores(self.forward(h[a:b]), tokens[a:b], top, vocab_limit, out.rows(a, b))
+        if rows == 0:
+            return out
+        with K.on_device_of(h):
+            weight, rt = self.linear.weight, self.linear.rt
+            if (self.linear.fast is not None and rows > SCORE_STORED
+                    and K.head_scores_supported(h, weight)):
+                K.head_scores(h, weight, limit, self.scale, self.softcap, tokens.contiguous(), top,
+                              *out.tensors(), rt.error_word)
+                return out
+            for a in range(0, rows, SCORE_BAND):
+                b = min(rows, a + SCORE_BAND)
+                token_scores(self.forward(h[a:b]), tokens[a:b], top, vocab_limit, out.rows(a, b))
         return out
 
 
