@@ -18,12 +18,12 @@ MB_DEFINE_LAST_ERROR
 
 #define HS_THREADS 192
 #define HS_BK 64
-#define HS_STAGES 5
+#define HS_STAGES 6
 #define HS_HALF (128 * HS_BK * 2)            // one CTA's rows of an operand in a stage
+#define HS_PAIRS 96                          // CTA pairs at most
 #define HS_BLOCKS 64                         // row blocks of 256 of a launch at most
-#define HS_LIST (MB_SCORES_TOP * 128 * 8)    // a key list for each of 128 rows
 #define HS_STAGED (4 * 32 * 128)             // 32 values of 32 rows for each epilogue warp
-#define HS_SMEM (1024 + HS_STAGES * 2 * HS_HALF + 256 + HS_LIST + HS_STAGED)
+#define HS_SMEM (1024 + HS_STAGES * 2 * HS_HALF + 256 + HS_STAGED)
 
 // A band: `blocks` row blocks from `first` on, each in `strips` strips of `width` ids, tiles of `tile`
 struct HeadPlan {
@@ -57,44 +57,42 @@ struct HeadWalk {
   __device__ __forceinline__ void step() { n += plan.tile[band]; }
 };
 
-// A row's greatest values so far: `top` keys in shared memory in no order (`list`: this row's first
-// one, 128 keys from one to the next), of which the least is known.
-struct TopList {
-  uint32_t list;
-  int top, worst;
-  TopKey least;
-  float bar;        // what a value has to pass: not (x <= bar); a NaN while the list has room
-
-  __device__ __forceinline__ void clear(uint32_t at, int top_) {
-    list = at;
-    top = top_;
-    worst = 0;
-    least = 0;
-    bar = __uint_as_float(0x7fc00000u);
-    for (int i = 0; i < top; ++i) put(i, 0);
-  }
-  __device__ __forceinline__ void put(int i, TopKey k) const {
-    asm volatile("st.shared.b64 [%0], %1;" ::"r"(list + i * 1024), "l"(k) : "memory");
-  }
-  __device__ __forceinline__ TopKey get(int i) const {
-    TopKey k;
-    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(k) : "r"(list + i * 1024) : "memory");
-    return k;
-  }
-  __device__ __forceinline__ void offer(TopKey k) {
-    if (k <= least) return;
-    put(worst, k);
-    TopKey m = ~(TopKey)0;
-    int at = 0;
-#pragma unroll 4
-    for (int i = 0; i < top; ++i) {
-      const TopKey c = get(i);
-      if (c < m) { m = c; at = i; }
+// A row's greatest values so far, in order, in registers: the last `top` of N places (what stands above
+// them is never passed). A value goes in where it is greater, so the first of equals stays ahead.
+template <int N> struct TopList {
+  float v[N];
+  int id[N];
+  __device__ __forceinline__ void clear(int top) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = i < N - top ? INFINITY : -INFINITY;
+      id[i] = -1;
     }
-    least = m;
-    worst = at;
-    bar = m == 0 ? __uint_as_float(0x7fc00000u) : key_value(m);
   }
+  __device__ __forceinline__ float bar() const { return v[N - 1]; }
+  __device__ __forceinline__ void offer(float x, int i) {
+    bool past[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) past[k] = x > v[k];
+#pragma unroll
+    for (int k = N - 1; k > 0; --k) {
+      v[k] = past[k - 1] ? v[k - 1] : past[k] ? x : v[k];
+      id[k] = past[k - 1] ? id[k - 1] : past[k] ? i : id[k];
+    }
+    v[0] = past[0] ? x : v[0];
+    id[0] = past[0] ? i : id[0];
+  }
+  __device__ __forceinline__ void write(TopKey* keys, int top) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (k >= N - top) keys[k - (N - top)] = id[k] < 0 ? 0 : key_of(v[k], id[k]);
+  }
+};
+template <> struct TopList<0> {
+  __device__ __forceinline__ void clear(int) {}
+  __device__ __forceinline__ float bar() const { return 0.f; }
+  __device__ __forceinline__ void offer(float, int) {}
+  __device__ __forceinline__ void write(TopKey*, int) const {}
 };
 
 // 32 columns of this thread's lane
@@ -110,15 +108,33 @@ __device__ __forceinline__ void load32(uint32_t taddr, float* x) {
     x[16 + j] = __uint_as_float(b[j]);
   }
 }
-// The head's factor and cap, as the kernels behind a stored product apply them
+// cap tanh(x / cap). For |u| up to 1 the continued fraction u / (1 + u^2 / (3 + u^2 / (5 + ...)))
+// (Lambert) cut behind the 9 gives u (945 + 105 u^2 + u^4) / (945 + 420 u^2 + 15 u^4), off by less than
+// 4 units of 2^-24; beyond it the exponential's form is exact enough. tanhf and a division took 3 us a tile of
+// 256 ids and, for the zeros of rows that are not there, 9.
+__device__ __forceinline__ float capped_small(float x, float cap, float by) {
+  const float u = x * by, z = u * u;
+  return cap * __fdividef(u * fmaf(z, z + 105.f, 945.f), fmaf(z, fmaf(z, 15.f, 420.f), 945.f));
+}
 __device__ __forceinline__ void shape32(float* x, float scale, float cap) {
   if (scale != 1.f) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) x[j] *= scale;
   }
   if (cap > 0.f) {
+    const float by = 1.f / cap;
+    bool small = true;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) x[j] = cap * tanhf(x[j] / cap);
+    for (int j = 0; j < 32; ++j) small = small && fabsf(x[j]) <= cap;
+    if (__all_sync(0xffffffffu, small)) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) x[j] = capped_small(x[j], cap, by);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        x[j] = fabsf(x[j]) > cap ? cap * tanh_of_2xlog2e(x[j] * by * 2.8853900817779268f)
+                                 : capped_small(x[j], cap, by);
+    }
   }
 }
 __device__ __forceinline__ float max32(const float* x) {
@@ -128,6 +144,7 @@ __device__ __forceinline__ float max32(const float* x) {
   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
+template <int N>
 __global__ void __launch_bounds__(HS_THREADS, 1)
 head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ HeadPlan plan, int rows, int limit, int K, float scale,
@@ -141,7 +158,7 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   const uint32_t full0 = bars, empty0 = bars + 8 * HS_STAGES;
   const uint32_t acc_full0 = bars + 16 * HS_STAGES, acc_empty0 = acc_full0 + 16;
   const uint32_t slot = acc_empty0 + 16;
-  const uint32_t lists = bars + 256, staged = lists + HS_LIST;
+  const uint32_t staged = bars + 256;
   volatile uint32_t* slot_ptr = (volatile uint32_t*)(smem_raw + (slot - raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -223,15 +240,16 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       const int in_block = (int)rank * 128 + lane_row, row = walk.row0() + in_block;
       const int token = row < rows ? tokens[row] : -1;
       float m = -INFINITY, s = 0.f, t = 0.f;     // the row's mass
-      TopList list;
-      list.clear(lists + lane_row * 8, top);
+      TopList<N> list;
+      list.clear(top);
+      const bool idle = walk.row0() + (int)rank * 128 + q * 32 >= rows;    // none of the warp's rows is there
       for (; walk.n < walk.end; walk.step(), ++it) {
         const int b = it & 1, cols = walk.cols();
         mbar_wait(acc_full0 + 8 * b, (it >> 1) & 1, error, 64);
         tc_fence_after_sync();
         float tile_s = 0.f, tile_t = 0.f;        // the tile's part, over the same maximum
 #pragma unroll 1
-        for (int c = 0; c < cols; c += 32) {
+        for (int c = 0; c < (idle ? 0 : cols); c += 32) {
           float x[32];
           load32(tmem + b * 256 + ((uint32_t)(q * 32) << 16) + c, x);
           const int n = min(32, cols - c), id0 = walk.n + c;
@@ -260,22 +278,21 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             for (int j = 0; j < 32; ++j)
               if (off == (unsigned)j && j < n) given[row] = x[j];
           }
-          if (top > 0 && __any_sync(0xffffffffu, !(most <= list.bar))) {
+          if (N > 0 && __any_sync(0xffffffffu, most > list.bar())) {
             // Which values pass is a bit each; a lane takes its own one after another. They are read
             // again from shared memory, where a register could not be named by a number.
             unsigned pass = 0;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + j * 128), "f"(x[j]) : "memory");
-              if (!(x[j] <= list.bar)) pass |= 1u << j;
+              if (x[j] > list.bar()) pass |= 1u << j;
             }
-            if (n < 32) pass &= (1u << n) - 1;
             while (pass) {
               const int j = __ffs(pass) - 1;
               pass &= pass - 1;
               float y;
               asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(mine + j * 128) : "memory");
-              list.offer(key_of(y, id0 + j));
+              list.offer(y, id0 + j);
             }
             __syncwarp();
           }
@@ -293,7 +310,7 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         const int strips = plan.strips[walk.band];
         const size_t part = plan.part0[walk.band] + ((size_t)walk.block * 256 + in_block) * strips + walk.strip;
         mass[part] = {m, s, t};
-        for (int i = 0; i < top; ++i) keys[part * top + i] = list.get(i);
+        list.write(keys + part * top, top);
       }
     }
   }
@@ -303,35 +320,81 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
-// A block a row joins its strips.
-__global__ void __launch_bounds__(128)
+// A warp a row joins its strips: their masses, and `top` times the greatest of the heads of their keys,
+// which are in order. A lane has the strips lane, lane + 32 and lane + 64.
+__global__ void __launch_bounds__(32)
 head_join_kernel(const __grid_constant__ HeadPlan plan, const Mass* __restrict__ mass,
                  const TopKey* __restrict__ keys, int top, const float* __restrict__ given, int limit,
                  const int* __restrict__ tokens, ScoreOut out) {
   mb_grid_wait();
   mb_grid_launch_next();
-  const int row = blockIdx.x;
+  extern __shared__ TopKey sh_keys[];
+  const int row = blockIdx.x, lane = threadIdx.x;
+  const int token = tokens[row];
+  const float logit = token >= 0 && token < limit ? given[row] : __uint_as_float(0x7fc00000u);
   int band = 0, block = row >> 8;
   while (band + 1 < plan.bands && block >= plan.first[band + 1]) ++band;
   block -= plan.first[band];
   const int strips = plan.strips[band];
   const size_t part = plan.part0[band] + ((size_t)block * 256 + (row & 255)) * strips;
-  const int token = tokens[row];
-  const bool ok = token >= 0 && token < limit;
-  join_parts(mass + part, keys + part * top, strips, top, ok ? given[row] : __uint_as_float(0x7fc00000u),
-             row, out);
+  for (int i = lane; i < strips * top; i += 32) sh_keys[i] = keys[part * top + i];
+  Mass v = mass_none();
+#pragma unroll
+  for (int i = 0; i < HS_PAIRS / 32; ++i)
+    if (lane + 32 * i < strips) v = mass_join(v, mass[part + lane + 32 * i]);
+  v = mass_warp(v);
+  __syncwarp();
+  TopKey mine = 0;
+  if (top > 0) {
+    int head[HS_PAIRS / 32];
+    TopKey next[HS_PAIRS / 32];
+#pragma unroll
+    for (int i = 0; i < HS_PAIRS / 32; ++i) {
+      head[i] = (lane + 32 * i) * top;
+      next[i] = lane + 32 * i < strips ? sh_keys[head[i]] : 0;
+    }
+    for (int j = 0; j < top; ++j) {
+      TopKey best = 0;
+#pragma unroll
+      for (int i = 0; i < HS_PAIRS / 32; ++i)
+        if (next[i] > best) best = next[i];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const TopKey c = __shfl_xor_sync(0xffffffffu, best, o);
+        if (c > best) best = c;
+      }
+      if (best == 0) break;
+#pragma unroll
+      for (int i = 0; i < HS_PAIRS / 32; ++i)
+        if (next[i] == best) {
+          ++head[i];
+          next[i] = head[i] < (lane + 32 * i + 1) * top ? sh_keys[head[i]] : 0;
+        }
+      if (lane == j) mine = best;
+    }
+  }
+  finish_row(v, logit, mine, top, row, out);
 }
 
-static cudaError_t allow_smem() {
-  static unsigned long long done = 0;
-  return mb_allow_smem((const void*)head_scores_kernel, HS_SMEM, &done);
+typedef void (*HeadKernel)(CUtensorMap, CUtensorMap, HeadPlan, int, int, int, float, float, const int*, int,
+                           float*, Mass*, TopKey*, int*);
+// The kernel whose lists have room for `top` keys
+static int head_form(int top) { return (top + 7) / 8; }
+static HeadKernel head_kernel(int form) {
+  static const HeadKernel kernels[5] = {head_scores_kernel<0>, head_scores_kernel<8>, head_scores_kernel<16>,
+                                        head_scores_kernel<24>, head_scores_kernel<32>};
+  return kernels[form];
+}
+static cudaError_t allow_smem(int form) {
+  static unsigned long long done[5] = {0, 0, 0, 0, 0};
+  return mb_allow_smem((const void*)head_kernel(form), HS_SMEM, &done[form]);
 }
 
 // How many CTA pairs the device runs at once (0: the kernel cannot run here)
 static int head_pairs(int sms) {
   static int pairs = -1;
   if (pairs >= 0) return pairs;
-  if (allow_smem() != cudaSuccess) {
+  if (allow_smem(4) != cudaSuccess) {
     cudaGetLastError();
     return pairs = 0;
   }
@@ -347,11 +410,12 @@ static int head_pairs(int sms) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, head_scores_kernel, &cfg) != cudaSuccess) {
+  if (cudaOccupancyMaxActiveClusters(&n, head_kernel(4), &cfg) != cudaSuccess) {
     cudaGetLastError();
     n = 0;
   }
-  return pairs = n > sms / 2 ? sms / 2 : n;
+  n = n > sms / 2 ? sms / 2 : n;
+  return pairs = n > HS_PAIRS ? HS_PAIRS : n;
 }
 
 // Ids of a strip where `blocks` row blocks share the pairs, a multiple of 16
@@ -423,7 +487,8 @@ MB_EXPORT int mb_head_scores(const void* A, int lda, const void* W, int rows, in
   if (scratch_bytes < mb_head_scores_scratch(rows, limit, top, sms))
     MB_FAIL("mb_head_scores: %lld bytes of scratch", scratch_bytes);
   const int pairs = head_pairs(sms);
-  if (cudaError_t e = allow_smem()) MB_FAIL("mb_head_scores: %s", cudaGetErrorString(e));
+  const int form = head_form(top);
+  if (cudaError_t e = allow_smem(form)) MB_FAIL("mb_head_scores: %s", cudaGetErrorString(e));
   cudaStream_t s = (cudaStream_t)stream;
   CUtensorMap tmB;
   if (!mb_make_map_bf16(&tmB, W, limit, K, K, 128, "mb_head_scores weight")) return -1;
@@ -441,13 +506,15 @@ MB_EXPORT int mb_head_scores(const void* A, int lda, const void* W, int rows, in
     int used = 0;
     for (int i = 0; i < plan.bands; ++i)
       if (plan.blocks[i] * plan.strips[i] > used) used = plan.blocks[i] * plan.strips[i];
-    cudaError_t e = mb_launch_clusters(head_scores_kernel, dim3(2 * used), dim3(HS_THREADS), HS_SMEM, s,
+    cudaError_t e = mb_launch_clusters(head_kernel(form), dim3(2 * used), dim3(HS_THREADS), HS_SMEM, s,
                                        2, tmA, tmB, plan, n, limit, K, scale, cap, tokens + r0, top,
                                        given, mass, keys, error);
     if (e != cudaSuccess) MB_FAIL("mb_head_scores: %s", cudaGetErrorString(e));
     const ScoreOut out = {logprobs + r0, entropy + r0, top_ids + (size_t)r0 * top,
                           top_logprobs + (size_t)r0 * top};
-    mb_launch(head_join_kernel, dim3(n), dim3(128), 0, s, plan, mass, keys, top, given, limit,
+    int strips = 0;
+    for (int i = 0; i < plan.bands; ++i) strips = plan.strips[i] > strips ? plan.strips[i] : strips;
+    mb_launch(head_join_kernel, dim3(n), dim3(32), (size_t)strips * top * 8, s, plan, mass, keys, top, given, limit,
               tokens + r0, out);
   }
   MB_CHECK_LAUNCH("mb_head_scores");

@@ -1,80 +1,273 @@
 // Log probabilities of given tokens, with the entropy and the greatest alternatives, from float32
-// logits (the formulas stand in scores.cuh). Two kernels: a row is cut into chunks, whose blocks leave
-// a mass and their greatest keys; a block a row joins them.
+// logits (the formulas stand in scores.cuh). Every logit is read once, into registers: a cluster of up
+// to eight CTAs shares a row, a thread holds 40 values of it at a time. Over the block's maximum they are
+// added up; the alternatives are picked out by a bar that at least `top` of them pass. The cluster's
+// first CTA then joins the parts through distributed shared memory, so that one launch does it all.
 #include "scores.cuh"
 
 MB_DEFINE_LAST_ERROR
 
-#define SCORE_THREADS 256
-#define SCORE_CHUNK 8192
+#define SC_THREADS 512
+#define SC_WARPS (SC_THREADS / 32)
+#define SC_EACH 40                      // values of a thread in a round
+#define SC_ROUND (SC_THREADS * SC_EACH)
+#define SC_ROOM 512                     // values that may pass the bar; more are picked one by one
+#define SC_CLUSTER 8
 
-__global__ void __launch_bounds__(SCORE_THREADS)
-score_chunks_kernel(const float* __restrict__ logits, size_t stride, int V, int chunk, int top,
-                    Mass* __restrict__ mass, TopKey* __restrict__ keys) {
-  mb_grid_wait();
-  mb_grid_launch_next();
-  __shared__ Mass sh_mass[SCORE_THREADS / 32];
-  __shared__ TopKey sh_key[SCORE_THREADS / 32];
-  const int i0 = blockIdx.y * chunk, n = min(chunk, V - i0);
-  const float* x = logits + (size_t)blockIdx.x * stride + i0;
-  const size_t part = (size_t)blockIdx.x * gridDim.y + blockIdx.y;
-  Mass v = mass_none();
-  for (int i = threadIdx.x; i < n; i += SCORE_THREADS) v.m = fmaxf(v.m, x[i]);
-  const float m = v.m == -INFINITY ? 0.f : v.m;
-  for (int i = threadIdx.x; i < n; i += SCORE_THREADS) mass_add(x[i], m, v.s, v.t);
-  v = block_mass(v, sh_mass);
-  if (threadIdx.x == 0) mass[part] = v;
-  TopKey last = ~(TopKey)0;
-  for (int j = 0; j < top; ++j) {
-    TopKey best = 0;
-    for (int i = threadIdx.x; i < n; i += SCORE_THREADS) {
-      const TopKey k = key_of(x[i], i0 + i);
-      if (k < last && k > best) best = k;
+__device__ __forceinline__ uint32_t sc_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t sc_at_leader(const void* p) {     // this shared address in CTA 0
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(0));
+  return r;
+}
+__device__ __forceinline__ void sc_put(uint32_t at, TopKey v) {
+  asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
+}
+__device__ __forceinline__ void sc_put(uint32_t at, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+__device__ __forceinline__ void sc_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void sc_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The `top`-th greatest of the warp's values, each lane one
+__device__ __forceinline__ float warp_nth(float v, int top) {
+  const int lane = threadIdx.x & 31;
+  int above = 0;
+#pragma unroll
+  for (int i = 1; i < 32; ++i) above += __shfl_sync(0xffffffffu, v, (lane + i) & 31) > v;
+  float least = above < top ? v : INFINITY;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+  return least;
+}
+
+struct ScShared {
+  float best[SC_WARPS], bar[SC_WARPS], s[SC_WARPS], t[SC_WARPS];
+  TopKey found[SC_ROOM + MB_SCORES_TOP], sorted[MB_SCORES_TOP], pick[SC_WARPS];
+  int count;
+  // of the cluster's first CTA: every CTA's part
+  Mass mass[SC_CLUSTER];
+  TopKey keys[SC_CLUSTER][MB_SCORES_TOP];
+};
+
+// Values `base` .. of the row's part x[0 .. n): value 4 i + j of a thread is at `place`
+template <bool WIDE>
+__device__ __forceinline__ int sc_place(int base, int k) {
+  return WIDE ? base + 4 * ((k >> 2) * SC_THREADS + threadIdx.x) + (k & 3) : base + k * SC_THREADS + threadIdx.x;
+}
+template <bool WIDE>
+__device__ __forceinline__ void sc_load(const float* __restrict__ x, int base, int n, float* v) {
+  if (WIDE) {
+#pragma unroll
+    for (int i = 0; i < SC_EACH; i += 4) {
+      const int at = sc_place<true>(base, i);
+      if (at + 4 <= n) {
+        const float4 f = *(const float4*)(x + at);
+        v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i + j] = at + j < n ? x[at + j] : -INFINITY;
+      }
     }
-    last = block_key_max(best, sh_key);
-    if (threadIdx.x == 0) keys[part * top + j] = last;
+  } else {
+#pragma unroll
+    for (int i = 0; i < SC_EACH; ++i) {
+      const int at = sc_place<false>(base, i);
+      v[i] = at < n ? x[at] : -INFINITY;
+    }
   }
 }
 
-__global__ void __launch_bounds__(128)
-score_join_kernel(const Mass* __restrict__ mass, const TopKey* __restrict__ keys, int parts, int top,
-                  const float* __restrict__ logits, size_t stride, int V,
-                  const int* __restrict__ tokens, ScoreOut out) {
-  mb_grid_wait();
-  mb_grid_launch_next();
-  const int row = blockIdx.x, t = tokens[row];
-  const bool ok = t >= 0 && t < V;
-  const size_t part = (size_t)row * parts;
-  join_parts(mass + part, keys + part * top, parts, top,
-             ok ? logits[(size_t)row * stride + t] : __uint_as_float(0x7fc00000u), row, out);
+template <bool WIDE, bool TOP>
+__device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int id0, int top, ScShared& sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float m = -INFINITY, s = 0.f, t = 0.f, bar = -INFINITY;
+  int held = 0;                        // keys in sh.sorted
+  for (int base = 0; base < n; base += SC_ROUND) {
+    float v[SC_EACH];
+    sc_load<WIDE>(x, base, n, v);
+    float best = v[0];
+#pragma unroll
+    for (int i = 1; i < SC_EACH; ++i) best = fmaxf(best, v[i]);
+    const float nth = TOP ? warp_nth(best, top) : 0.f;
+    best = warp_max(best);
+    __syncthreads();                   // the round before has read what is written next
+    if (lane == 0) {
+      sh.best[warp] = best;
+      if (TOP) sh.bar[warp] = nth;
+    }
+    if (TOP && threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    float most = m;
+#pragma unroll
+    for (int w = 0; w < SC_WARPS; ++w) {
+      most = fmaxf(most, sh.best[w]);
+      if (TOP) bar = fmaxf(bar, sh.bar[w]);
+    }
+    const Mass before = mass_over({m, s, t}, most);
+    m = most, s = before.s, t = before.t;
+    const float at = m == -INFINITY ? 0.f : m;
+    float ps[4] = {0.f, 0.f, 0.f, 0.f}, pt[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < SC_EACH; ++i) mass_add(v[i], at, ps[i & 3], pt[i & 3]);
+    s += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+    t += (pt[0] + pt[1]) + (pt[2] + pt[3]);
+    if (!TOP) continue;
+    // What passes the bar: at least `top` of the block's values do (each warp's bar is passed by its
+    // own), unless so many are not above -infinity.
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < SC_EACH; ++i) mine += v[i] >= bar && v[i] > -INFINITY;
+    if (mine) {
+      int to = atomicAdd(&sh.count, mine);
+      if (to + mine <= SC_ROOM) {
+#pragma unroll
+        for (int i = 0; i < SC_EACH; ++i)
+          if (v[i] >= bar && v[i] > -INFINITY) sh.found[to++] = key_of(v[i], id0 + sc_place<WIDE>(base, i));
+      }
+    }
+    __syncthreads();
+    const int passed = sh.count;
+    if (passed <= SC_ROOM) {
+      // every key's place is the number of keys above it
+      const int all = passed + held;
+      if (threadIdx.x < held) sh.found[passed + threadIdx.x] = sh.sorted[threadIdx.x];
+      __syncthreads();
+      for (int i = threadIdx.x; i < all; i += SC_THREADS) {
+        const TopKey k = sh.found[i];
+        int above = 0;
+        for (int j = 0; j < all; ++j) above += sh.found[j] > k;
+        if (above < top) sh.sorted[above] = k;
+      }
+      held = min(top, all);
+    } else {
+      // many equal values, or many large ones side by side: the greatest below the last, `top` times
+      TopKey old = threadIdx.x < held ? sh.sorted[threadIdx.x] : 0, last = ~(TopKey)0;
+      for (int r = 0; r < top; ++r) {
+        TopKey k = old < last ? old : 0;
+#pragma unroll
+        for (int i = 0; i < SC_EACH; ++i) {
+          if (!(v[i] > -INFINITY)) continue;
+          const TopKey c = key_of(v[i], id0 + sc_place<WIDE>(base, i));
+          if (c < last && c > k) k = c;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const TopKey c = __shfl_xor_sync(0xffffffffu, k, o);
+          if (c > k) k = c;
+        }
+        __syncthreads();
+        if (lane == 0) sh.pick[warp] = k;
+        __syncthreads();
+        last = 0;
+        for (int w = 0; w < SC_WARPS; ++w)
+          if (sh.pick[w] > last) last = sh.pick[w];
+        if (threadIdx.x == 0) sh.sorted[r] = last;
+      }
+      held = top;
+    }
+    __syncthreads();
+    if (held == top) bar = fmaxf(bar, key_value(sh.sorted[top - 1]));
+  }
+  // keys that are not there are 0
+  if (TOP && threadIdx.x < top && threadIdx.x >= held) sh.sorted[threadIdx.x] = 0;
+  s = warp_sum(s);
+  t = warp_sum(t);
+  if (lane == 0) sh.s[warp] = s, sh.t[warp] = t;
+  __syncthreads();
+  s = warp_sum(lane < SC_WARPS ? sh.s[lane] : 0.f);
+  t = warp_sum(lane < SC_WARPS ? sh.t[lane] : 0.f);
+  return {m, s, t};
 }
 
-static int chunks_of(int V) { return (V + SCORE_CHUNK - 1) / SCORE_CHUNK; }
-
-// bytes of scratch that mb_token_scores needs
-MB_EXPORT long long mb_token_scores_scratch(int rows, int V, int top) {
-  return (long long)rows * chunks_of(V) * (long long)(16 + 8 * top);
+template <bool TOP>
+__global__ void __launch_bounds__(SC_THREADS, 2)
+token_scores_kernel(const float* __restrict__ logits, size_t stride, int V, int parts, int per,
+                    const int* __restrict__ tokens, int top, ScoreOut out) {
+  mb_grid_wait();
+  mb_grid_launch_next();
+  __shared__ ScShared sh;
+  if (parts > 1) sc_arrive();                  // every CTA of the cluster has begun: see the wait
+  const int row = blockIdx.x / parts, part = parts > 1 ? (int)sc_rank() : 0;
+  const float* x = logits + (size_t)row * stride;
+  float given = __uint_as_float(0x7fc00000u);
+  if (part == 0 && threadIdx.x == 0) {         // asked for ahead of everything
+    const int token = tokens[row];
+    if (token >= 0 && token < V) given = x[token];
+  }
+  const int i0 = part * per, n = max(0, min(per, V - i0));
+  const bool wide = ((uintptr_t)x & 15) == 0;
+  const Mass v = wide ? sc_part<true, TOP>(x + i0, n, i0, top, sh) : sc_part<false, TOP>(x + i0, n, i0, top, sh);
+  if (parts > 1) {
+    sc_wait();
+    if (threadIdx.x == 0) {
+      sc_put(sc_at_leader(&sh.mass[part].m), v.m);
+      sc_put(sc_at_leader(&sh.mass[part].s), v.s);
+      sc_put(sc_at_leader(&sh.mass[part].t), v.t);
+    }
+    if (TOP && threadIdx.x < top) sc_put(sc_at_leader(&sh.keys[part][threadIdx.x]), sh.sorted[threadIdx.x]);
+    sc_arrive();
+    sc_wait();
+    if (part > 0) return;
+  } else {
+    if (threadIdx.x == 0) sh.mass[0] = v;
+    if (TOP && threadIdx.x < top) sh.keys[0][threadIdx.x] = sh.sorted[threadIdx.x];
+    __syncthreads();
+  }
+  if (threadIdx.x >= 32) return;
+  const int lane = threadIdx.x;
+  Mass all = lane < parts ? sh.mass[lane] : mass_none();
+#pragma unroll
+  for (int o = SC_CLUSTER / 2; o > 0; o >>= 1)
+    all = mass_join(all, {__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.s, o),
+                          __shfl_xor_sync(0xffffffffu, all.t, o)});
+  TopKey mine = 0;
+  if (TOP) {      // every part's keys are in order: the greatest of their heads, `top` times
+    int head = 0;
+    for (int j = 0; j < top; ++j) {
+      const TopKey k = lane < parts && head < top ? sh.keys[lane][head] : 0;
+      TopKey best = k;
+#pragma unroll
+      for (int o = SC_CLUSTER / 2; o > 0; o >>= 1) {
+        const TopKey c = __shfl_xor_sync(0xffffffffu, best, o);
+        if (c > best) best = c;
+      }
+      best = __shfl_sync(0xffffffffu, best, 0);
+      if (k == best) ++head;
+      if (lane == j) mine = best;
+    }
+  }
+  all = {__shfl_sync(0xffffffffu, all.m, 0), __shfl_sync(0xffffffffu, all.s, 0), __shfl_sync(0xffffffffu, all.t, 0)};
+  finish_row(all, __shfl_sync(0xffffffffu, given, 0), mine, top, row, out);
 }
 
 // For every row r of logits [rows, V] (`stride` values from row to row): logprobs[r] of tokens[r] (NaN
 // where that is no token below V), entropy[r], and the `top` greatest values' ids and log
-// probabilities. scratch: mb_token_scores_scratch bytes, 16-byte aligned.
+// probabilities. `sms`: the device's multiprocessors.
 MB_EXPORT int mb_token_scores(const float* logits, long long stride, int rows, int V,
                               const int* tokens, int top, float* logprobs, float* entropy,
-                              int* top_ids, float* top_logprobs, void* scratch,
-                              long long scratch_bytes, void* stream) {
+                              int* top_ids, float* top_logprobs, int sms, void* stream) {
   if (rows <= 0) return 0;
   if (V <= 0 || top < 0 || top > MB_SCORES_TOP || top > V)
     MB_FAIL("mb_token_scores: %d alternatives of a vocabulary of %d", top, V);
-  if (scratch_bytes < mb_token_scores_scratch(rows, V, top))
-    MB_FAIL("mb_token_scores: %lld bytes of scratch", scratch_bytes);
-  cudaStream_t s = (cudaStream_t)stream;
-  const int parts = chunks_of(V);
-  TopKey* keys = (TopKey*)scratch;
-  Mass* mass = (Mass*)(keys + (size_t)rows * parts * top);
-  mb_launch(score_chunks_kernel, dim3(rows, parts), dim3(SCORE_THREADS), 0, s, logits, (size_t)stride,
-            V, SCORE_CHUNK, top, mass, keys);
-  mb_launch(score_join_kernel, dim3(rows), dim3(128), 0, s, mass, keys, parts, top, logits,
-            (size_t)stride, V, tokens, ScoreOut{logprobs, entropy, top_ids, top_logprobs});
-  MB_CHECK_LAUNCH("mb_token_scores");
+  // few rows: parts of at least 2,048 values, for the latency; many: whole rounds
+  const int least = (long long)rows * 2 < sms ? 2048 : SC_ROUND;
+  int parts = 1;
+  while (parts < SC_CLUSTER && (long long)parts * least < V) parts *= 2;
+  if ((long long)rows * parts > 0x7fffffffll) MB_FAIL("mb_token_scores: %d rows in one call", rows);
+  const int per = (((V + parts - 1) / parts) + 3) & ~3;
+  const ScoreOut out = {logprobs, entropy, top_ids, top_logprobs};
+  cudaError_t e = mb_launch_clusters(top > 0 ? token_scores_kernel<true> : token_scores_kernel<false>,
+                                     dim3(rows * parts), dim3(SC_THREADS), 0, (cudaStream_t)stream, parts,
+                                     logits, (size_t)stride, V, parts, per, tokens, top, out);
+  if (e != cudaSuccess) MB_FAIL("mb_token_scores: %s", cudaGetErrorString(e));
+  return 0;
 }

@@ -63,35 +63,6 @@ __device__ __forceinline__ float key_value(TopKey k) {
   const uint32_t p = (uint32_t)(k >> 32);
   return p == 0u ? __uint_as_float(0x7fc00000u) : __uint_as_float(p & 0x80000000u ? p ^ 0x80000000u : ~p);
 }
-__device__ __forceinline__ TopKey key_max_warp(TopKey k) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const TopKey c = __shfl_xor_sync(0xffffffffu, k, o);
-    if (c > k) k = c;
-  }
-  return k;
-}
-
-__device__ TopKey block_key_max(TopKey k, TopKey* sh) {
-  k = key_max_warp(k);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  __syncthreads();
-  if (lane == 0) sh[warp] = k;
-  __syncthreads();
-  k = sh[0];
-  for (int w = 1; w < warps; ++w)
-    if (sh[w] > k) k = sh[w];
-  return k;
-}
-__device__ Mass block_mass(Mass v, Mass* sh) {
-  v = mass_warp(v);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  if (lane == 0) sh[warp] = v;
-  __syncthreads();
-  v = sh[0];
-  for (int w = 1; w < warps; ++w) v = mass_join(v, sh[w]);
-  return v;
-}
 
 struct ScoreOut {
   float *logprobs, *entropy;
@@ -99,32 +70,31 @@ struct ScoreOut {
   float* top_logprobs;
 };
 
-// A block of 128 threads joins the parts of a row: their masses and, in any order, their keys.
-// `given`: the given token's logit, a NaN where there is none.
-__device__ void join_parts(const Mass* mass, const TopKey* keys, int parts, int top, float given, int row,
-                           const ScoreOut& out) {
-  __shared__ Mass sh_mass[4];
-  __shared__ TopKey sh_key[4];
-  Mass v = mass_none();
-  for (int p = threadIdx.x; p < parts; p += 128) v = mass_join(v, mass[p]);
-  v = block_mass(v, sh_mass);
+// What a warp makes of a row's joined mass, the given token's logit (a NaN where there is none) and the
+// greatest values in order, lane j the j-th's key (0 where there are no more). What is left then are
+// values of -infinity (or NaNs, in a row whose numbers are NaN anyway): the lowest ids that are not listed.
+__device__ __forceinline__ void finish_row(Mass v, float given, TopKey key, int top, int row,
+                                           const ScoreOut& out) {
+  const int lane = threadIdx.x & 31;
   const float ln_s = logf(v.s);
-  if (threadIdx.x == 0) {
+  if (lane == 0) {
     out.logprobs[row] = given - v.m - ln_s;
     const float h = ln_s - v.t / v.s;
     out.entropy[row] = h < 0.f ? 0.f : h;
   }
-  TopKey last = ~(TopKey)0;
-  for (int j = 0; j < top; ++j) {
-    TopKey best = 0;
-    for (int i = threadIdx.x; i < parts * top; i += 128) {
-      const TopKey k = keys[i];
-      if (k < last && k > best) best = k;
+  if (top == 0) return;
+  int id = key_id(key);
+  float value = key_value(key);
+  const unsigned found = __ballot_sync(0xffffffffu, key != 0 && lane < top);
+  for (int j = __popc(found), next = 0; j < top; ++j, ++next) {
+    while (__any_sync(0xffffffffu, lane < j && id == next)) ++next;
+    if (lane == j) {
+      id = next;
+      value = -INFINITY;
     }
-    last = block_key_max(best, sh_key);
-    if (threadIdx.x == 0) {
-      out.top_ids[(size_t)row * top + j] = key_id(last);
-      out.top_logprobs[(size_t)row * top + j] = key_value(last) - v.m - ln_s;
-    }
+  }
+  if (lane < top) {
+    out.top_ids[(size_t)row * top + lane] = id;
+    out.top_logprobs[(size_t)row * top + lane] = value - v.m - ln_s;
   }
 }

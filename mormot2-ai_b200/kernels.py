@@ -1513,14 +1513,10 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int, logprobs:
     assert top_ids.numel() == top_logprobs.numel() == rows * top
     for t in (logprobs, entropy, top_ids, top_logprobs):
         _contig(t, "an output of the scores")
-    f, _ = _functions.get("mb_token_scores_scratch") or _function(
-        "scores", "mb_token_scores_scratch", [_i, _i, _i], _ll)
-    scratch = torch.empty(f(rows, V, top), dtype=torch.uint8, device=logits.device)
     _call("scores", "mb_token_scores",
-          [_vp, _ll, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
+          [_vp, _ll, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp],
           _ptr(logits), logits.stride(0), rows, V, _ptr(tokens), top, _ptr(logprobs),
-          _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs), _ptr(scratch), scratch.numel(),
-          _stream(), launches=2)
+          _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs), _sms(), _stream())
 
 
 def head_scores_supported(h: torch.Tensor, w: torch.Tensor) -> bool:

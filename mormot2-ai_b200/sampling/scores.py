@@ -26,9 +26,9 @@ class TokenScore:
 class Scores:
     """One entry a row: ``logprobs`` and ``entropy`` (natural logarithms, float32 [rows]); the ids
     (int32) and log probabilities of the alternatives [rows, top], the most probable first and the
-    lowest id first among equals. A row with a NaN or a positive infinity among its logits, or with
-    nothing but negative infinities, has no distribution: its numbers are NaN (its ids are still in the
-    order of the logits, a NaN last)."""
+    lowest id first among equals; negative infinities and NaNs come last, the lowest id first. A row
+    with a NaN or a positive infinity among its logits, or with nothing but negative infinities, has
+    no distribution: its numbers are NaN."""
     logprobs: torch.Tensor
     entropy: torch.Tensor
     top_ids: torch.Tensor

@@ -3,10 +3,9 @@ import numpy as np
 
 
 def order(row):
-    """Ids in the order of alternatives: the greater value first, the lowest id among equals, a NaN
-    last."""
-    value = np.where(np.isnan(row), -np.inf, row)
-    return np.lexsort((np.arange(len(row)), np.isnan(row), -value))
+    """Ids in the order of alternatives: the greater value first, the lowest id among equals; a NaN
+    stands with the negative infinities."""
+    return np.argsort(-np.where(np.isnan(row), -np.inf, row), kind="stable")
 
 
 def scores(x, tokens, top):
