@@ -267,11 +267,7 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             tile_s = tile_part.s, tile_t = tile_part.t;
           }
           const float at = m == -INFINITY ? 0.f : m;
-          float ps[4] = {0.f, 0.f, 0.f, 0.f}, pt[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < 32; ++j) mass_add(x[j], at, ps[j & 3], pt[j & 3]);
-          tile_s += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-          tile_t += (pt[0] + pt[1]) + (pt[2] + pt[3]);
+          mass_add<32>(x, at, tile_s, tile_t);
           const unsigned off = (unsigned)token - (unsigned)id0;
           if (__any_sync(0xffffffffu, off < (unsigned)n)) {
 #pragma unroll

@@ -7,7 +7,7 @@
 
 MB_DEFINE_LAST_ERROR
 
-#define SC_THREADS 512
+#define SC_THREADS 256
 #define SC_WARPS (SC_THREADS / 32)
 #define SC_EACH 40                      // values of a thread in a round
 #define SC_ROUND (SC_THREADS * SC_EACH)
@@ -49,10 +49,16 @@ __device__ __forceinline__ float warp_nth(float v, int top) {
   return least;
 }
 
+#define SC_FEW 8       // alternatives up to which the warps' bars are near enough
+
 struct ScShared {
-  float best[SC_WARPS], bar[SC_WARPS], s[SC_WARPS], t[SC_WARPS];
-  TopKey found[SC_ROOM + MB_SCORES_TOP], sorted[MB_SCORES_TOP], pick[SC_WARPS];
-  int count;
+  float best[2][SC_WARPS], bar[2][SC_WARPS], s[SC_WARPS], t[SC_WARPS];
+  alignas(16) uint32_t place[SC_ROOM];      // of the keys that passed the bar, and their ids
+  uint32_t id[SC_ROOM];
+  alignas(16) uint32_t heads[SC_THREADS];   // the threads' greatest values that passed the warps' bars
+  TopKey sorted[MB_SCORES_TOP], pick[SC_WARPS];
+  int taken[MB_SCORES_TOP], count, n_heads, equal[2];
+  uint32_t least;
   // of the cluster's first CTA: every CTA's part
   Mass mass[SC_CLUSTER];
   TopKey keys[SC_CLUSTER][MB_SCORES_TOP];
@@ -86,95 +92,141 @@ __device__ __forceinline__ void sc_load(const float* __restrict__ x, int base, i
   }
 }
 
+// How many of list[0 .. n) are above p
+__device__ __forceinline__ int sc_above(const uint32_t* list, int n, uint32_t p) {
+  int above = 0, j = 0;
+  for (; j + 4 <= n; j += 4) {
+    const uint4 q = *(const uint4*)(list + j);
+    above += (q.x > p) + (q.y > p) + (q.z > p) + (q.w > p);
+  }
+  for (; j < n; ++j) above += list[j] > p;
+  return above;
+}
+
+// The `top` greatest of the `n` keys in sh.place and sh.id, in order into sh.sorted: a key's place is the
+// number of keys above it, for which its value alone is looked at unless two are equal.
+__device__ __forceinline__ void sc_sort(int n, int top, int parity, ScShared& sh) {
+  for (int i = threadIdx.x; i < n; i += SC_THREADS) {
+    const uint32_t p = sh.place[i];
+    const int above = sc_above(sh.place, n, p);
+    if (above < top) {
+      sh.sorted[above] = (TopKey)p << 32 | sh.id[i];
+      if (atomicAdd(&sh.taken[above], 1) > 0) sh.equal[parity] = 1;
+    }
+  }
+  __syncthreads();
+  if (!sh.equal[parity]) return;
+  for (int i = threadIdx.x; i < n; i += SC_THREADS) {
+    const TopKey k = (TopKey)sh.place[i] << 32 | sh.id[i];
+    int above = 0;
+    for (int j = 0; j < n; ++j) above += ((TopKey)sh.place[j] << 32 | sh.id[j]) > k;
+    if (above < top) sh.sorted[above] = k;
+  }
+  __syncthreads();
+}
+
+// The same of the round's values themselves, where so many passed that they were not noted (many equal
+// ones, or large ones side by side): the greatest below the last one, `top` times. They are read again.
+__device__ __noinline__ void sc_pick(const float* __restrict__ x, int base, int n, int id0, int held, int top,
+                                     ScShared& sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const TopKey old = threadIdx.x < held ? sh.sorted[threadIdx.x] : 0;
+  const int end = min(n, base + SC_ROUND);
+  TopKey last = ~(TopKey)0;
+  for (int r = 0; r < top; ++r) {
+    TopKey k = old < last ? old : 0;
+    for (int i = base + threadIdx.x; i < end; i += SC_THREADS) {
+      const float v = x[i];
+      const TopKey c = v > -INFINITY ? key_of(v, id0 + i) : 0;
+      if (c < last && c > k) k = c;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const TopKey c = __shfl_xor_sync(0xffffffffu, k, o);
+      if (c > k) k = c;
+    }
+    __syncthreads();
+    if (lane == 0) sh.pick[warp] = k;
+    __syncthreads();
+    last = 0;
+    for (int w = 0; w < SC_WARPS; ++w)
+      if (sh.pick[w] > last) last = sh.pick[w];
+    if (threadIdx.x == 0) sh.sorted[r] = last;
+  }
+  __syncthreads();
+}
+
 template <bool WIDE, bool TOP>
 __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int id0, int top, ScShared& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float m = -INFINITY, s = 0.f, t = 0.f, bar = -INFINITY;
+  float m = -INFINITY, s = 0.f, t = 0.f;
+  float bar = -3.402823466e38f;        // the lowest finite value: -infinity and NaN never pass
   int held = 0;                        // keys in sh.sorted
-  for (int base = 0; base < n; base += SC_ROUND) {
+  for (int base = 0, parity = 0; base < n; base += SC_ROUND, parity ^= 1) {
     float v[SC_EACH];
     sc_load<WIDE>(x, base, n, v);
     float best = v[0];
 #pragma unroll
     for (int i = 1; i < SC_EACH; ++i) best = fmaxf(best, v[i]);
-    const float nth = TOP ? warp_nth(best, top) : 0.f;
-    best = warp_max(best);
-    __syncthreads();                   // the round before has read what is written next
+    const float most_warp = warp_max(best);
+    const float nth = TOP ? top == 1 ? most_warp : warp_nth(best, top) : 0.f;
     if (lane == 0) {
-      sh.best[warp] = best;
-      if (TOP) sh.bar[warp] = nth;
+      sh.best[parity][warp] = most_warp;
+      if (TOP) sh.bar[parity][warp] = nth;
     }
-    if (TOP && threadIdx.x == 0) sh.count = 0;
+    if (TOP) {
+      if (threadIdx.x < MB_SCORES_TOP) sh.taken[threadIdx.x] = 0;
+      if (threadIdx.x == 0) sh.count = held, sh.n_heads = 0, sh.equal[parity] = 0, sh.least = ~0u;
+      if (threadIdx.x < held) {
+        sh.place[threadIdx.x] = (uint32_t)(sh.sorted[threadIdx.x] >> 32);
+        sh.id[threadIdx.x] = (uint32_t)sh.sorted[threadIdx.x];
+      }
+    }
     __syncthreads();
     float most = m;
 #pragma unroll
     for (int w = 0; w < SC_WARPS; ++w) {
-      most = fmaxf(most, sh.best[w]);
-      if (TOP) bar = fmaxf(bar, sh.bar[w]);
+      most = fmaxf(most, sh.best[parity][w]);
+      if (TOP) bar = fmaxf(bar, sh.bar[parity][w]);
     }
-    const Mass before = mass_over({m, s, t}, most);
-    m = most, s = before.s, t = before.t;
-    const float at = m == -INFINITY ? 0.f : m;
-    float ps[4] = {0.f, 0.f, 0.f, 0.f}, pt[4] = {0.f, 0.f, 0.f, 0.f};
+    if (TOP && top > SC_FEW) {
+      // The `top`-th of the threads' greatest values is a bar too, and one that few others pass; only those
+      // that pass the warps' bars (at least `top` do, if so many are finite) can be above it.
+      const uint32_t p = key_place(best);
+      if (best >= bar) sh.heads[atomicAdd(&sh.n_heads, 1)] = p;
+      __syncthreads();
+      const int heads = sh.n_heads;
+      if (best >= bar && sc_above(sh.heads, heads, p) < top) atomicMin(&sh.least, p);
+      __syncthreads();
+      if (heads >= top) bar = fmaxf(bar, key_value((TopKey)sh.least << 32));
+    }
+    if (TOP && best >= bar) {
+      int mine = 0;
 #pragma unroll
-    for (int i = 0; i < SC_EACH; ++i) mass_add(v[i], at, ps[i & 3], pt[i & 3]);
-    s += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-    t += (pt[0] + pt[1]) + (pt[2] + pt[3]);
-    if (!TOP) continue;
-    // What passes the bar: at least `top` of the block's values do (each warp's bar is passed by its
-    // own), unless so many are not above -infinity.
-    int mine = 0;
-#pragma unroll
-    for (int i = 0; i < SC_EACH; ++i) mine += v[i] >= bar && v[i] > -INFINITY;
-    if (mine) {
+      for (int i = 0; i < SC_EACH; ++i) mine += v[i] >= bar;
       int to = atomicAdd(&sh.count, mine);
       if (to + mine <= SC_ROOM) {
 #pragma unroll
         for (int i = 0; i < SC_EACH; ++i)
-          if (v[i] >= bar && v[i] > -INFINITY) sh.found[to++] = key_of(v[i], id0 + sc_place<WIDE>(base, i));
+          if (v[i] >= bar) {
+            sh.place[to] = key_place(v[i]);
+            sh.id[to++] = ~(uint32_t)(id0 + sc_place<WIDE>(base, i));
+          }
       }
     }
+    const Mass before = mass_over({m, s, t}, most);
+    m = most, s = before.s, t = before.t;
+    mass_add<SC_EACH>(v, m == -INFINITY ? 0.f : m, s, t);
+    if (!TOP) continue;
     __syncthreads();
-    const int passed = sh.count;
+    const int passed = sh.count;       // the keys held among them
     if (passed <= SC_ROOM) {
-      // every key's place is the number of keys above it
-      const int all = passed + held;
-      if (threadIdx.x < held) sh.found[passed + threadIdx.x] = sh.sorted[threadIdx.x];
-      __syncthreads();
-      for (int i = threadIdx.x; i < all; i += SC_THREADS) {
-        const TopKey k = sh.found[i];
-        int above = 0;
-        for (int j = 0; j < all; ++j) above += sh.found[j] > k;
-        if (above < top) sh.sorted[above] = k;
-      }
-      held = min(top, all);
+      sc_sort(passed, top, parity, sh);
+      held = min(top, passed);
     } else {
-      // many equal values, or many large ones side by side: the greatest below the last, `top` times
-      TopKey old = threadIdx.x < held ? sh.sorted[threadIdx.x] : 0, last = ~(TopKey)0;
-      for (int r = 0; r < top; ++r) {
-        TopKey k = old < last ? old : 0;
-#pragma unroll
-        for (int i = 0; i < SC_EACH; ++i) {
-          if (!(v[i] > -INFINITY)) continue;
-          const TopKey c = key_of(v[i], id0 + sc_place<WIDE>(base, i));
-          if (c < last && c > k) k = c;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const TopKey c = __shfl_xor_sync(0xffffffffu, k, o);
-          if (c > k) k = c;
-        }
-        __syncthreads();
-        if (lane == 0) sh.pick[warp] = k;
-        __syncthreads();
-        last = 0;
-        for (int w = 0; w < SC_WARPS; ++w)
-          if (sh.pick[w] > last) last = sh.pick[w];
-        if (threadIdx.x == 0) sh.sorted[r] = last;
-      }
+      sc_pick(x, base, n, id0, held, top, sh);
       held = top;
     }
-    __syncthreads();
     if (held == top) bar = fmaxf(bar, key_value(sh.sorted[top - 1]));
   }
   // keys that are not there are 0
@@ -189,7 +241,7 @@ __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int 
 }
 
 template <bool TOP>
-__global__ void __launch_bounds__(SC_THREADS, 2)
+__global__ void __launch_bounds__(SC_THREADS, 4)
 token_scores_kernel(const float* __restrict__ logits, size_t stride, int V, int parts, int per,
                     const int* __restrict__ tokens, int top, ScoreOut out) {
   mb_grid_wait();

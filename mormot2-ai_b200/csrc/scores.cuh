@@ -12,6 +12,18 @@ struct Mass {
   float m, s, t;
 };
 
+__device__ __forceinline__ f32_pair pair_add(f32_pair a, f32_pair b) {
+  f32_pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^y; what is below the smallest normal value is 0
+__device__ __forceinline__ float exp2_fast(float y) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
+  return e;
+}
+
 __device__ __forceinline__ Mass mass_none() { return {-INFINITY, 0.f, 0.f}; }
 
 // The two parts' mass over their common maximum. A part that weighs nothing beside the other (all of it
@@ -27,12 +39,23 @@ __device__ __forceinline__ Mass mass_join(Mass a, Mass b) {
   return {m, a.s + b.s, a.t + b.t};
 }
 
-// One value onto a mass whose maximum `m` is final (0 stands for -infinity): -infinity adds nothing,
-// a NaN stays.
-__device__ __forceinline__ void mass_add(float x, float m, float& s, float& t) {
-  const float d = x - m, e = __expf(d);
-  s += e;
-  t = fmaf(e, fmaxf(d, -1e30f), t);
+// N values onto the sums over a maximum `m` that is final (0 stands for -infinity): s += sum e^(x - m),
+// t += sum e^(x - m) (x - m), two at a time. -infinity adds nothing, a NaN stays.
+template <int N> __device__ __forceinline__ void mass_add(const float* x, float m, float& s, float& t) {
+  const f32_pair less = pair_of(-m, -m);
+  f32_pair ps[2] = {0, 0}, pt[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    f32_pair d = pair_add(pair_of(x[j], x[j + 1]), less), y = d;
+    pair_mul(y, pair_of(1.4426950408889634f, 1.4426950408889634f));
+    const f32_pair e = pair_of(exp2_fast(pair_half(y, 0)), exp2_fast(pair_half(y, 1)));
+    d = pair_of(fmaxf(pair_half(d, 0), -1e30f), fmaxf(pair_half(d, 1), -1e30f));
+    ps[(j >> 1) & 1] = pair_add(ps[(j >> 1) & 1], e);
+    pair_fma(pt[(j >> 1) & 1], e, d);
+  }
+  const f32_pair a = pair_add(ps[0], ps[1]), b = pair_add(pt[0], pt[1]);
+  s += pair_half(a, 0) + pair_half(a, 1);
+  t += pair_half(b, 0) + pair_half(b, 1);
 }
 
 __device__ __forceinline__ Mass mass_warp(Mass v) {
