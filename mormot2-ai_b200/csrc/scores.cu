@@ -39,10 +39,9 @@ __device__ __forceinline__ void sc_wait() {
 
 // The `top`-th greatest of the warp's values, each lane one
 __device__ __forceinline__ float warp_nth(float v, int top) {
-  const int lane = threadIdx.x & 31;
   int above = 0;
 #pragma unroll
-  for (int i = 1; i < 32; ++i) above += __shfl_sync(0xffffffffu, v, (lane + i) & 31) > v;
+  for (int i = 1; i < 32; ++i) above += __shfl_xor_sync(0xffffffffu, v, i) > v;
   float least = above < top ? v : INFINITY;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
@@ -52,13 +51,14 @@ __device__ __forceinline__ float warp_nth(float v, int top) {
 #define SC_FEW 8       // alternatives up to which the warps' bars are near enough
 
 struct ScShared {
-  float best[2][SC_WARPS], bar[2][SC_WARPS], s[SC_WARPS], t[SC_WARPS];
-  alignas(16) uint32_t place[SC_ROOM];      // of the keys that passed the bar, and their ids
-  uint32_t id[SC_ROOM];
+  float best[SC_WARPS], bar[SC_WARPS];
+  alignas(16) uint32_t place[SC_ROOM];      // of the keys held, in order, and of those that passed the bar
+  uint32_t id[SC_ROOM];                     // and their ids
   alignas(16) uint32_t heads[SC_THREADS];   // the threads' greatest values that passed the warps' bars
   TopKey sorted[MB_SCORES_TOP], pick[SC_WARPS];
-  int taken[MB_SCORES_TOP], count, n_heads, equal[2];
+  int taken[MB_SCORES_TOP], passed[3], n_heads, equal[2];
   uint32_t least;
+  Mass part[SC_WARPS];
   // of the cluster's first CTA: every CTA's part
   Mass mass[SC_CLUSTER];
   TopKey keys[SC_CLUSTER][MB_SCORES_TOP];
@@ -104,18 +104,22 @@ __device__ __forceinline__ int sc_above(const uint32_t* list, int n, uint32_t p)
 }
 
 // The `top` greatest of the `n` keys in sh.place and sh.id, in order into sh.sorted: a key's place is the
-// number of keys above it, for which its value alone is looked at unless two are equal.
-__device__ __forceinline__ void sc_sort(int n, int top, int parity, ScShared& sh) {
+// number of keys above it, for which its value alone is looked at unless two are equal. `turn` counts
+// these calls (sh.taken and sh.equal[turn & 1] are 0 before each).
+__device__ __forceinline__ void sc_sort(int n, int top, int turn, ScShared& sh) {
   for (int i = threadIdx.x; i < n; i += SC_THREADS) {
     const uint32_t p = sh.place[i];
     const int above = sc_above(sh.place, n, p);
     if (above < top) {
       sh.sorted[above] = (TopKey)p << 32 | sh.id[i];
-      if (atomicAdd(&sh.taken[above], 1) > 0) sh.equal[parity] = 1;
+      if (atomicAdd(&sh.taken[above], 1) > 0) sh.equal[turn & 1] = 1;
     }
   }
   __syncthreads();
-  if (!sh.equal[parity]) return;
+  const int equal = sh.equal[turn & 1];
+  if (threadIdx.x < MB_SCORES_TOP) sh.taken[threadIdx.x] = 0;
+  if (threadIdx.x == 0) sh.equal[(turn + 1) & 1] = 0;
+  if (!equal) return;
   for (int i = threadIdx.x; i < n; i += SC_THREADS) {
     const TopKey k = (TopKey)sh.place[i] << 32 | sh.id[i];
     int above = 0;
@@ -156,56 +160,53 @@ __device__ __noinline__ void sc_pick(const float* __restrict__ x, int base, int 
   __syncthreads();
 }
 
+// What a CTA finds in its part of a row, x[0 .. n) with ids from id0 on: the mass (every thread has it),
+// and in sh.sorted the greatest `top` keys in order, 0 where there are no more finite values.
+//
+// The first round sets a bar that few values pass and the `top` greatest do: each warp knows the `top`-th
+// of its 32 threads' greatest values, and the highest of these bars holds for the block. From then on
+// the bar is the `top`-th greatest value so far, which hardly any value passes, and a round costs what the
+// sums cost, and one barrier. Each thread's sums are over the greatest value that it has seen itself.
 template <bool WIDE, bool TOP>
 __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int id0, int top, ScShared& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float m = -INFINITY, s = 0.f, t = 0.f;
+  Mass mine = mass_none();
   float bar = -3.402823466e38f;        // the lowest finite value: -infinity and NaN never pass
-  int held = 0;                        // keys in sh.sorted
-  for (int base = 0, parity = 0; base < n; base += SC_ROUND, parity ^= 1) {
+  int held = 0, turn = 0, third = 0;   // keys in sh.sorted; sorts; the round's counter of three
+  if (TOP) {
+    if (threadIdx.x < MB_SCORES_TOP) sh.taken[threadIdx.x] = 0;
+    if (threadIdx.x == 0) sh.passed[0] = sh.n_heads = sh.equal[0] = 0, sh.least = ~0u;
+  }
+  for (int base = 0; base < n; base += SC_ROUND) {
     float v[SC_EACH];
     sc_load<WIDE>(x, base, n, v);
     float best = v[0];
 #pragma unroll
     for (int i = 1; i < SC_EACH; ++i) best = fmaxf(best, v[i]);
-    const float most_warp = warp_max(best);
-    const float nth = TOP ? top == 1 ? most_warp : warp_nth(best, top) : 0.f;
-    if (lane == 0) {
-      sh.best[parity][warp] = most_warp;
-      if (TOP) sh.bar[parity][warp] = nth;
-    }
-    if (TOP) {
-      if (threadIdx.x < MB_SCORES_TOP) sh.taken[threadIdx.x] = 0;
-      if (threadIdx.x == 0) sh.count = held, sh.n_heads = 0, sh.equal[parity] = 0, sh.least = ~0u;
-      if (threadIdx.x < held) {
-        sh.place[threadIdx.x] = (uint32_t)(sh.sorted[threadIdx.x] >> 32);
-        sh.id[threadIdx.x] = (uint32_t)sh.sorted[threadIdx.x];
+    if (TOP && base == 0) {
+      const float nth = top == 1 ? warp_max(best) : warp_nth(best, top);
+      if (lane == 0) sh.bar[warp] = nth;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < SC_WARPS; ++w) bar = fmaxf(bar, sh.bar[w]);
+      if (top > SC_FEW) {
+        // The `top`-th of all threads' greatest values is a bar as well, which fewer pass; only those that
+        // pass the warps' bars (at least `top` do, if so many are finite) can be above it.
+        const uint32_t p = key_place(best);
+        if (best >= bar) sh.heads[atomicAdd(&sh.n_heads, 1)] = p;
+        __syncthreads();
+        const int heads = sh.n_heads;
+        if (best >= bar && sc_above(sh.heads, heads, p) < top) atomicMin(&sh.least, p);
+        __syncthreads();
+        if (heads >= top) bar = key_value((TopKey)sh.least << 32);
       }
     }
-    __syncthreads();
-    float most = m;
-#pragma unroll
-    for (int w = 0; w < SC_WARPS; ++w) {
-      most = fmaxf(most, sh.best[parity][w]);
-      if (TOP) bar = fmaxf(bar, sh.bar[parity][w]);
-    }
-    if (TOP && top > SC_FEW) {
-      // The `top`-th of the threads' greatest values is a bar too, and one that few others pass; only those
-      // that pass the warps' bars (at least `top` do, if so many are finite) can be above it.
-      const uint32_t p = key_place(best);
-      if (best >= bar) sh.heads[atomicAdd(&sh.n_heads, 1)] = p;
-      __syncthreads();
-      const int heads = sh.n_heads;
-      if (best >= bar && sc_above(sh.heads, heads, p) < top) atomicMin(&sh.least, p);
-      __syncthreads();
-      if (heads >= top) bar = fmaxf(bar, key_value((TopKey)sh.least << 32));
-    }
     if (TOP && best >= bar) {
-      int mine = 0;
+      int many = 0;
 #pragma unroll
-      for (int i = 0; i < SC_EACH; ++i) mine += v[i] >= bar;
-      int to = atomicAdd(&sh.count, mine);
-      if (to + mine <= SC_ROOM) {
+      for (int i = 0; i < SC_EACH; ++i) many += v[i] >= bar;
+      int to = held + atomicAdd(&sh.passed[third], many);
+      if (to + many <= SC_ROOM) {
 #pragma unroll
         for (int i = 0; i < SC_EACH; ++i)
           if (v[i] >= bar) {
@@ -214,30 +215,34 @@ __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int 
           }
       }
     }
-    const Mass before = mass_over({m, s, t}, most);
-    m = most, s = before.s, t = before.t;
-    mass_add<SC_EACH>(v, m == -INFINITY ? 0.f : m, s, t);
+    if (best > mine.m) mine = mass_over(mine, best);
+    mass_add<SC_EACH>(v, mine.m == -INFINITY ? 0.f : mine.m, mine.s, mine.t);
     if (!TOP) continue;
+    const int next = third == 2 ? 0 : third + 1;
+    if (threadIdx.x == 0) sh.passed[next] = 0;      // read two rounds ago, a barrier ago by all
     __syncthreads();
-    const int passed = sh.count;       // the keys held among them
-    if (passed <= SC_ROOM) {
-      sc_sort(passed, top, parity, sh);
-      held = min(top, passed);
+    const int passed = sh.passed[third];
+    third = next;
+    if (passed == 0) continue;
+    if (held + passed <= SC_ROOM) {
+      sc_sort(held + passed, top, turn++, sh);
+      held = min(top, held + passed);
     } else {
       sc_pick(x, base, n, id0, held, top, sh);
       held = top;
     }
-    if (held == top) bar = fmaxf(bar, key_value(sh.sorted[top - 1]));
+    if (threadIdx.x < held) {
+      sh.place[threadIdx.x] = (uint32_t)(sh.sorted[threadIdx.x] >> 32);
+      sh.id[threadIdx.x] = (uint32_t)sh.sorted[threadIdx.x];
+    }
+    // what is to come has to be above the last of them (the next value up: equal ones come later)
+    if (held == top) bar = key_value(((sh.sorted[top - 1] >> 32) + 1) << 32);
   }
-  // keys that are not there are 0
   if (TOP && threadIdx.x < top && threadIdx.x >= held) sh.sorted[threadIdx.x] = 0;
-  s = warp_sum(s);
-  t = warp_sum(t);
-  if (lane == 0) sh.s[warp] = s, sh.t[warp] = t;
+  mine = mass_warp(mine);
+  if (lane == 0) sh.part[warp] = mine;
   __syncthreads();
-  s = warp_sum(lane < SC_WARPS ? sh.s[lane] : 0.f);
-  t = warp_sum(lane < SC_WARPS ? sh.t[lane] : 0.f);
-  return {m, s, t};
+  return mass_warp(lane < SC_WARPS ? sh.part[lane] : mass_none());
 }
 
 template <bool TOP>
@@ -310,10 +315,14 @@ MB_EXPORT int mb_token_scores(const float* logits, long long stride, int rows, i
   if (rows <= 0) return 0;
   if (V <= 0 || top < 0 || top > MB_SCORES_TOP || top > V)
     MB_FAIL("mb_token_scores: %d alternatives of a vocabulary of %d", top, V);
-  // few rows: parts of at least 2,048 values, for the latency; many: whole rounds
-  const int least = (long long)rows * 2 < sms ? 2048 : SC_ROUND;
+  // As many parts a row as make the rounds of CTAs (four run on a multiprocessor) the shortest, a part's
+  // start and end counting as 4,096 values, and none of less than 2,048.
   int parts = 1;
-  while (parts < SC_CLUSTER && (long long)parts * least < V) parts *= 2;
+  long long cost = 0;
+  for (int p = 1; p <= SC_CLUSTER && (p == 1 || (long long)V >= 2048ll * p); p *= 2) {
+    const long long c = ((long long)rows * p + 4 * sms - 1) / (4 * sms) * ((V + p - 1) / p + 4096);
+    if (p == 1 || c < cost) cost = c, parts = p;
+  }
   if ((long long)rows * parts > 0x7fffffffll) MB_FAIL("mb_token_scores: %d rows in one call", rows);
   const int per = (((V + parts - 1) / parts) + 3) & ~3;
   const ScoreOut out = {logprobs, entropy, top_ids, top_logprobs};
