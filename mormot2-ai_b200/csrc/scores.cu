@@ -1,7 +1,7 @@
 // Log probabilities of given tokens, with the entropy and the greatest alternatives, from float32
 // logits (the formulas stand in scores.cuh). Every logit is read once, into registers: a cluster of up
-// to eight CTAs shares a row, a thread holds 40 values of it at a time. Over the block's maximum they are
-// added up; the alternatives are picked out by a bar that at least `top` of them pass. The cluster's
+// to eight CTAs shares a row, a thread holds 24 or 40 values of it at a time. They are added up over the
+// thread's maximum; the alternatives are picked out by a bar that at least `top` of them pass. The cluster's
 // first CTA then joins the parts through distributed shared memory, so that one launch does it all.
 #include "scores.cuh"
 
@@ -9,8 +9,6 @@ MB_DEFINE_LAST_ERROR
 
 #define SC_THREADS 256
 #define SC_WARPS (SC_THREADS / 32)
-#define SC_EACH 40                      // values of a thread in a round
-#define SC_ROUND (SC_THREADS * SC_EACH)
 #define SC_ROOM 512                     // values that may pass the bar; more are picked one by one
 #define SC_CLUSTER 8
 
@@ -69,11 +67,11 @@ template <bool WIDE>
 __device__ __forceinline__ int sc_place(int base, int k) {
   return WIDE ? base + 4 * ((k >> 2) * SC_THREADS + threadIdx.x) + (k & 3) : base + k * SC_THREADS + threadIdx.x;
 }
-template <bool WIDE>
+template <int EACH, bool WIDE>
 __device__ __forceinline__ void sc_load(const float* __restrict__ x, int base, int n, float* v) {
   if (WIDE) {
 #pragma unroll
-    for (int i = 0; i < SC_EACH; i += 4) {
+    for (int i = 0; i < EACH; i += 4) {
       const int at = sc_place<true>(base, i);
       if (at + 4 <= n) {
         const float4 f = *(const float4*)(x + at);
@@ -85,7 +83,7 @@ __device__ __forceinline__ void sc_load(const float* __restrict__ x, int base, i
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < SC_EACH; ++i) {
+    for (int i = 0; i < EACH; ++i) {
       const int at = sc_place<false>(base, i);
       v[i] = at < n ? x[at] : -INFINITY;
     }
@@ -131,11 +129,10 @@ __device__ __forceinline__ void sc_sort(int n, int top, int turn, ScShared& sh) 
 
 // The same of the round's values themselves, where so many passed that they were not noted (many equal
 // ones, or large ones side by side): the greatest below the last one, `top` times. They are read again.
-__device__ __noinline__ void sc_pick(const float* __restrict__ x, int base, int n, int id0, int held, int top,
+__device__ __noinline__ void sc_pick(const float* __restrict__ x, int base, int end, int id0, int held, int top,
                                      ScShared& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const TopKey old = threadIdx.x < held ? sh.sorted[threadIdx.x] : 0;
-  const int end = min(n, base + SC_ROUND);
   TopKey last = ~(TopKey)0;
   for (int r = 0; r < top; ++r) {
     TopKey k = old < last ? old : 0;
@@ -167,8 +164,9 @@ __device__ __noinline__ void sc_pick(const float* __restrict__ x, int base, int 
 // of its 32 threads' greatest values, and the highest of these bars holds for the block. From then on
 // the bar is the `top`-th greatest value so far, which hardly any value passes, and a round costs what the
 // sums cost, and one barrier. Each thread's sums are over the greatest value that it has seen itself.
-template <bool WIDE, bool TOP>
+template <int EACH, bool WIDE, bool TOP>
 __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int id0, int top, ScShared& sh) {
+  constexpr int ROUND = SC_THREADS * EACH;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Mass mine = mass_none();
   float bar = -3.402823466e38f;        // the lowest finite value: -infinity and NaN never pass
@@ -177,12 +175,12 @@ __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int 
     if (threadIdx.x < MB_SCORES_TOP) sh.taken[threadIdx.x] = 0;
     if (threadIdx.x == 0) sh.passed[0] = sh.n_heads = sh.equal[0] = 0, sh.least = ~0u;
   }
-  for (int base = 0; base < n; base += SC_ROUND) {
-    float v[SC_EACH];
-    sc_load<WIDE>(x, base, n, v);
+  for (int base = 0; base < n; base += ROUND) {
+    float v[EACH];
+    sc_load<EACH, WIDE>(x, base, n, v);
     float best = v[0];
 #pragma unroll
-    for (int i = 1; i < SC_EACH; ++i) best = fmaxf(best, v[i]);
+    for (int i = 1; i < EACH; ++i) best = fmaxf(best, v[i]);
     if (TOP && base == 0) {
       const float nth = top == 1 ? warp_max(best) : warp_nth(best, top);
       if (lane == 0) sh.bar[warp] = nth;
@@ -202,21 +200,23 @@ __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int 
       }
     }
     if (TOP && best >= bar) {
-      int many = 0;
+      // four at a time: hardly any pass
 #pragma unroll
-      for (int i = 0; i < SC_EACH; ++i) many += v[i] >= bar;
-      int to = held + atomicAdd(&sh.passed[third], many);
-      if (to + many <= SC_ROOM) {
+      for (int i = 0; i < EACH; i += 4) {
+        if (!(fmaxf(fmaxf(v[i], v[i + 1]), fmaxf(v[i + 2], v[i + 3])) >= bar)) continue;
 #pragma unroll
-        for (int i = 0; i < SC_EACH; ++i)
-          if (v[i] >= bar) {
-            sh.place[to] = key_place(v[i]);
-            sh.id[to++] = ~(uint32_t)(id0 + sc_place<WIDE>(base, i));
+        for (int j = i; j < i + 4; ++j)
+          if (v[j] >= bar) {
+            const int to = held + atomicAdd(&sh.passed[third], 1);
+            if (to < SC_ROOM) {
+              sh.place[to] = key_place(v[j]);
+              sh.id[to] = ~(uint32_t)(id0 + sc_place<WIDE>(base, j));
+            }
           }
       }
     }
     if (best > mine.m) mine = mass_over(mine, best);
-    mass_add<SC_EACH>(v, mine.m == -INFINITY ? 0.f : mine.m, mine.s, mine.t);
+    mass_add<EACH>(v, mine.m == -INFINITY ? 0.f : mine.m, mine.s, mine.t);
     if (!TOP) continue;
     const int next = third == 2 ? 0 : third + 1;
     if (threadIdx.x == 0) sh.passed[next] = 0;      // read two rounds ago, a barrier ago by all
@@ -228,7 +228,7 @@ __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int 
       sc_sort(held + passed, top, turn++, sh);
       held = min(top, held + passed);
     } else {
-      sc_pick(x, base, n, id0, held, top, sh);
+      sc_pick(x, base, min(n, base + ROUND), id0, held, top, sh);
       held = top;
     }
     if (threadIdx.x < held) {
@@ -245,8 +245,8 @@ __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int 
   return mass_warp(lane < SC_WARPS ? sh.part[lane] : mass_none());
 }
 
-template <bool TOP>
-__global__ void __launch_bounds__(SC_THREADS, 4)
+template <int EACH, int CTAS, bool TOP>
+__global__ void __launch_bounds__(SC_THREADS, CTAS)
 token_scores_kernel(const float* __restrict__ logits, size_t stride, int V, int parts, int per,
                     const int* __restrict__ tokens, int top, ScoreOut out) {
   mb_grid_wait();
@@ -262,7 +262,7 @@ token_scores_kernel(const float* __restrict__ logits, size_t stride, int V, int 
   }
   const int i0 = part * per, n = max(0, min(per, V - i0));
   const bool wide = ((uintptr_t)x & 15) == 0;
-  const Mass v = wide ? sc_part<true, TOP>(x + i0, n, i0, top, sh) : sc_part<false, TOP>(x + i0, n, i0, top, sh);
+  const Mass v = wide ? sc_part<EACH, true, TOP>(x + i0, n, i0, top, sh) : sc_part<EACH, false, TOP>(x + i0, n, i0, top, sh);
   if (parts > 1) {
     sc_wait();
     if (threadIdx.x == 0) {
@@ -315,18 +315,25 @@ MB_EXPORT int mb_token_scores(const float* logits, long long stride, int rows, i
   if (rows <= 0) return 0;
   if (V <= 0 || top < 0 || top > MB_SCORES_TOP || top > V)
     MB_FAIL("mb_token_scores: %d alternatives of a vocabulary of %d", top, V);
-  // As many parts a row as make the rounds of CTAs (four run on a multiprocessor) the shortest, a part's
-  // start and end counting as 4,096 values, and none of less than 2,048.
+  // Where a row in eight parts for each of a few rows fits the device at once, 40 values a thread make the
+  // fewest rounds; else 24 leave room for a fifth CTA on a multiprocessor, whose loads cover the others'
+  // barriers. 151,936 values, 5 alternatives, us with 40 | 24: 1 row 8.8 | 11.0, 64 rows 16 | 20, 300 rows
+  // 59 | 43, 2,048 rows 223 | 201; 2,048 rows of 4,000 values 31 | 26.
+  const bool few = (long long)rows * SC_CLUSTER <= 4 * sms;
+  // As many parts a row as make the rounds of CTAs the shortest, a part's start and end counting as 4,096
+  // values, and none of less than 2,048.
+  const int slots = (few ? 4 : 5) * sms;
   int parts = 1;
   long long cost = 0;
   for (int p = 1; p <= SC_CLUSTER && (p == 1 || (long long)V >= 2048ll * p); p *= 2) {
-    const long long c = ((long long)rows * p + 4 * sms - 1) / (4 * sms) * ((V + p - 1) / p + 4096);
+    const long long c = ((long long)rows * p + slots - 1) / slots * ((V + p - 1) / p + 4096);
     if (p == 1 || c < cost) cost = c, parts = p;
   }
-  if ((long long)rows * parts > 0x7fffffffll) MB_FAIL("mb_token_scores: %d rows in one call", rows);
   const int per = (((V + parts - 1) / parts) + 3) & ~3;
   const ScoreOut out = {logprobs, entropy, top_ids, top_logprobs};
-  cudaError_t e = mb_launch_clusters(top > 0 ? token_scores_kernel<true> : token_scores_kernel<false>,
+  const auto kernel = few ? top > 0 ? token_scores_kernel<40, 4, true> : token_scores_kernel<40, 4, false>
+                          : top > 0 ? token_scores_kernel<24, 5, true> : token_scores_kernel<24, 5, false>;
+  cudaError_t e = mb_launch_clusters(kernel,
                                      dim3(rows * parts), dim3(SC_THREADS), 0, (cudaStream_t)stream, parts,
                                      logits, (size_t)stride, V, parts, per, tokens, top, out);
   if (e != cudaSuccess) MB_FAIL("mb_token_scores: %s", cudaGetErrorString(e));

@@ -1505,18 +1505,23 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int, logprobs:
     where that is no id below V), the entropy, and the ids and log probabilities of the ``top``
     greatest logits, the lowest id first among equals. The outputs are contiguous."""
     rows, V = logits.shape
+    _score_outputs(rows, top, tokens, logprobs, entropy, top_ids, top_logprobs)
     assert logits.dtype == torch.float32 and (V == 1 or logits.stride(1) == 1)
-    assert tokens.dtype == torch.int32 and tokens.is_contiguous() and tokens.numel() == rows
-    assert logprobs.dtype == entropy.dtype == top_logprobs.dtype == torch.float32
-    assert top_ids.dtype == torch.int32
-    assert logprobs.numel() == entropy.numel() == rows
-    assert top_ids.numel() == top_logprobs.numel() == rows * top
-    for t in (logprobs, entropy, top_ids, top_logprobs):
-        _contig(t, "an output of the scores")
     _call("scores", "mb_token_scores",
           [_vp, _ll, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp],
           _ptr(logits), logits.stride(0), rows, V, _ptr(tokens), top, _ptr(logprobs),
           _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs), _sms(), _stream())
+
+
+def _score_outputs(rows: int, top: int, tokens: torch.Tensor, logprobs: torch.Tensor,
+                   entropy: torch.Tensor, top_ids: torch.Tensor, top_logprobs: torch.Tensor) -> None:
+    """Contiguous lists of the sizes that the scores' kernels write (and the tokens they read)."""
+    for t, dtype, n in ((tokens, torch.int32, rows), (logprobs, torch.float32, rows),
+                        (entropy, torch.float32, rows), (top_ids, torch.int32, rows * top),
+                        (top_logprobs, torch.float32, rows * top)):
+        if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
+            raise KernelError(f"scores of {rows} rows with {top} alternatives: {t.dtype} "
+                              f"{tuple(t.shape)}, not {n} contiguous values of {dtype}")
 
 
 def head_scores_supported(h: torch.Tensor, w: torch.Tensor) -> bool:
@@ -1535,13 +1540,8 @@ def head_scores(h: torch.Tensor, w: torch.Tensor, limit: int, scale: float, cap:
     > 0: cap tanh(x / cap)) for bfloat16 h [rows, K] and w [V, K], without storing them."""
     rows, Kd = h.shape
     assert w.shape[1] == Kd and h.stride(1) == 1 and 0 < limit <= w.shape[0]
-    assert tokens.dtype == torch.int32 and tokens.is_contiguous() and tokens.numel() == rows
-    assert logprobs.dtype == entropy.dtype == top_logprobs.dtype == torch.float32
-    assert top_ids.dtype == torch.int32 and logprobs.numel() == entropy.numel() == rows
-    assert top_ids.numel() == top_logprobs.numel() == rows * top
     _contig(w, "the weight")
-    for t in (logprobs, entropy, top_ids, top_logprobs):
-        _contig(t, "an output of the scores")
+    _score_outputs(rows, top, tokens, logprobs, entropy, top_ids, top_logprobs)
     f, _ = _functions.get("mb_head_scores_scratch") or _function(
         "head_scores", "mb_head_scores_scratch", [_i, _i, _i, _i], _ll)
     scratch = torch.empty(f(rows, limit, top, _sms()), dtype=torch.uint8, device=h.device)
@@ -1553,21 +1553,21 @@ def head_scores(h: torch.Tensor, w: torch.Tensor, limit: int, scale: float, cap:
 
 
 # ------------------------------------------------------------------------------ a step's arrays
-def _sequences(what: str, **lists) -> int:
-    """The length of int32 lists, which is the same for all of them, as is their device."""
-    first = next(iter(lists.values()))
-    n = first.numel()
-    for name, t in lists.items():
-        if (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.numel() != n
-                or t.device != first.device):
+def _lists(what: str, names: str, *tensors: torch.Tensor) -> int:
+    """The length of int32 lists, which has to be the same for all of them, as has their device."""
+    n, device = tensors[0].numel(), tensors[0].get_device()
+    for t in tensors:
+        if (t.dtype is not torch.int32 or t.numel() != n or t.dim() != 1 or not t.is_contiguous()
+                or t.get_device() != device):
+            name = names.split()[[u is t for u in tensors].index(True)]
             raise KernelError(f"{what}: {name} is {t.dtype} {tuple(t.shape)} on {t.device}, not a "
-                              f"contiguous int32 list of {n} on {first.device}")
+                              f"contiguous int32 list of {n} beside the others")
     return n
 
 
-def _same_device(what: str, first: torch.Tensor, *others: torch.Tensor) -> None:
+def _beside(what: str, first: torch.Tensor, *others: torch.Tensor) -> None:
     for t in others:
-        if t.device != first.device:
+        if t.get_device() != first.get_device():
             raise KernelError(f"{what}: tensors on {first.device} and on {t.device}")
 
 
@@ -1578,11 +1578,11 @@ def step_index(slots: torch.Tensor, past: torch.Tensor, new: torch.Tensor, seq_s
     rows and the end; per token its sequence, position and slot. The token arrays may be longer than
     the step (what lies behind it is left) or shorter (what does not fit is not written). All
     int32, on the device; nothing is read on the host."""
-    B = _sequences("step_index", slots=slots, past=past, new=new)
-    if _sequences("step_index", seq_start=seq_start) != B + 1:
+    B = _lists("step_index", "slots past new", slots, past, new)
+    T = _lists("step_index", "tok_seq tok_pos tok_slot", tok_seq, tok_pos, tok_slot)
+    if _lists("step_index", "seq_start", seq_start) != B + 1:
         raise KernelError(f"step_index: seq_start holds {seq_start.numel()} rows, not {B} + 1")
-    T = _sequences("step_index", tok_seq=tok_seq, tok_pos=tok_pos, tok_slot=tok_slot)
-    _same_device("step_index", slots, seq_start, tok_seq)
+    _beside("step_index", slots, seq_start, tok_seq)
     with on_device_of(slots):
         _call("step_index", "mb_step_index", [_vp, _vp, _vp, _i, _ll, _vp, _vp, _vp, _vp, _vp],
               _ptr(slots), _ptr(past), _ptr(new), B, T, _ptr(seq_start), _ptr(tok_seq),
@@ -1596,14 +1596,14 @@ def map_pages(table: torch.Tensor, slots: torch.Tensor, past: torch.Tensor, new:
     ``past[b] + new[b]`` positions take (at most ``ring_pages``, where that is above 0), sequence
     after sequence. Distinct slots. Entries outside the table are left, and so are those that ``pages``
     is too short for. All int32, on the device; nothing is read on the host."""
-    B = _sequences("map_pages", slots=slots, past=past, new=new, held=held)
-    N = _sequences("map_pages", pages=pages)
+    B = _lists("map_pages", "slots past new held", slots, past, new, held)
+    N = _lists("map_pages", "pages", pages)
     if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
         raise KernelError(f"map_pages: the table is {table.dtype} {tuple(table.shape)}, not a "
                           "contiguous int32 matrix")
     if ring_pages < 0:
         raise KernelError(f"map_pages: a ring of {ring_pages} pages")
-    _same_device("map_pages", slots, table, pages)
+    _beside("map_pages", slots, table, pages)
     with on_device_of(slots):
         _call("step_index", "mb_map_pages",
               [_vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _vp],

@@ -36,10 +36,14 @@ class Scores:
 
     @classmethod
     def empty(cls, rows: int, top: int, device) -> "Scores":
-        return cls(torch.empty(rows, dtype=torch.float32, device=device),
-                   torch.empty(rows, dtype=torch.float32, device=device),
-                   torch.empty((rows, top), dtype=torch.int32, device=device),
-                   torch.empty((rows, top), dtype=torch.float32, device=device))
+        return cls.beside(torch.empty(rows, dtype=torch.int32, device=device), rows, top)
+
+    @classmethod
+    def beside(cls, tokens: torch.Tensor, rows: int, top: int) -> "Scores":
+        """Scores on the device of ``tokens`` (int32)."""
+        logprobs = tokens.new_empty(rows, dtype=torch.float32)
+        return cls(logprobs, logprobs.new_empty(rows), tokens.new_empty((rows, top)),
+                   logprobs.new_empty((rows, top)))
 
     @classmethod
     def packed(cls, buffer: torch.Tensor, rows: int, top: int) -> "Scores":
@@ -84,16 +88,16 @@ def candidates(vocab: int, vocab_limit: Optional[int]) -> int:
 
 
 def check_top(top: int, vocab: int) -> int:
-    if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= min(K.TOP_SCORES, vocab):
+    if type(top) is not int or not 0 <= top <= K.TOP_SCORES or top > vocab:
         raise InferError(f"{top} alternatives: 0 to {min(K.TOP_SCORES, vocab)} can be had")
     return top
 
 
-def check_tokens(tokens: torch.Tensor, rows: int, device) -> None:
-    if (tokens.dtype != torch.int32 or tokens.dim() != 1 or tokens.shape[0] != rows
-            or tokens.device != device):
-        raise InferError(f"scores of {rows} rows on {device}: tokens are {tokens.dtype} "
-                         f"{tuple(tokens.shape)} on {tokens.device}, not int32 [{rows}] there")
+def check_tokens(tokens: torch.Tensor, rows: int, device: int) -> None:
+    if (tokens.dtype is not torch.int32 or tokens.dim() != 1 or tokens.numel() != rows
+            or tokens.get_device() != device):
+        raise InferError(f"scores of {rows} rows: tokens are {tokens.dtype} {tuple(tokens.shape)} on "
+                         f"{tokens.device}, not int32 [{rows}] beside them")
 
 
 def check_score(h: torch.Tensor, tokens: torch.Tensor, top: int, hidden: int, vocab: int,
@@ -105,7 +109,7 @@ def check_score(h: torch.Tensor, tokens: torch.Tensor, top: int, hidden: int, vo
                          f"rows of {hidden} values")
     vocab = candidates(vocab, vocab_limit)
     check_top(top, vocab)
-    check_tokens(tokens, h.shape[0], h.device)
+    check_tokens(tokens, h.shape[0], h.get_device())
     return vocab
 
 
@@ -116,23 +120,26 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     ``top``: alternatives, up to 32. ``vocab_limit``: only the ids below it take part. ``out``: to
     write into, contiguous, as ``Scores.empty`` makes it. Runs on the current stream of the logits'
     device and reads nothing back; what it needs besides is allocated for the call alone."""
-    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.shape[1] == 0:
+    if logits.dim() != 2 or logits.dtype is not torch.float32 or logits.shape[1] == 0:
         raise InferError(f"scores: logits are {logits.dtype} {tuple(logits.shape)}, not float32 "
                          "[rows, vocab]")
-    if logits.shape[1] > 1 and logits.stride(1) != 1:
+    rows, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
         raise InferError("scores: the logits of a row do not lie side by side")
-    rows, vocab = logits.shape[0], candidates(logits.shape[1], vocab_limit)
-    check_top(top, vocab)
-    check_tokens(tokens, rows, logits.device)
-    if vocab < logits.shape[1]:
+    if vocab_limit is not None:
+        vocab = candidates(vocab, vocab_limit)
         logits = logits[:, :vocab]
+    check_top(top, vocab)
+    check_tokens(tokens, rows, logits.get_device())
     if out is None:
-        out = Scores.empty(rows, top, logits.device)
-    elif out.top_ids.shape != (rows, top) or out.logprobs.device != logits.device:
+        out = Scores.beside(tokens, rows, top)
+    elif (out.top_ids.shape != (rows, top) or out.logprobs.get_device() != tokens.get_device()):
         raise InferError(f"scores of {rows} rows and {top} alternatives into {tuple(out.top_ids.shape)} "
                          f"on {out.logprobs.device}")
     if rows == 0:
         return out
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
     with K.on_device_of(logits):
-        K.token_scores(logits, tokens.contiguous(), top, *out.tensors())
+        K.token_scores(logits, tokens, top, out.logprobs, out.entropy, out.top_ids, out.top_logprobs)
     return out
