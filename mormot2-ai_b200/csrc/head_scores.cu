@@ -428,7 +428,7 @@ static void plan_bands(HeadPlan& plan, int blocks, int pairs, int limit) {
   for (int n = 1; n <= blocks; ++n) {
     best[n] = 0x7fffffff;
     for (int b = 1; b <= n && b <= pairs; ++b) {
-      const int cost = best[n - b] + strip_width(b, pairs, limit) + 64;
+      const int cost = best[n - b] + strip_width(b, pairs, limit) + 512;
       if (cost < best[n]) best[n] = cost, take[n] = b;
     }
   }

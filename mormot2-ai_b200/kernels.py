@@ -70,6 +70,13 @@ class _NoChange:
 _no_change = _NoChange()
 
 
+def elsewhere(device: int) -> bool:
+    """Whether a tensor's device (``get_device()``) is not the current one."""
+    if device < 0:
+        raise KernelError("a kernel was given a tensor that is not on the GPU")
+    return device != torch._C._cuda_getDevice()
+
+
 def on_device_of(t: torch.Tensor):
     """A ``with`` block whose launches go to the device of ``t`` and its current stream."""
     if not t.is_cuda:
@@ -1499,29 +1506,17 @@ def sample(logits: torch.Tensor, temperature: float, state_index: torch.Tensor,
 TOP_SCORES = 32          # alternatives of a row at most (MB_SCORES_TOP in csrc/scores.cuh)
 
 
-def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int, logprobs: torch.Tensor,
-                 entropy: torch.Tensor, top_ids: torch.Tensor, top_logprobs: torch.Tensor) -> None:
-    """Per row of ``logits`` [rows, V] (float32): the log probability of ``tokens[row]`` (int32; NaN
-    where that is no id below V), the entropy, and the ids and log probabilities of the ``top``
-    greatest logits, the lowest id first among equals. The outputs are contiguous."""
-    rows, V = logits.shape
-    _score_outputs(rows, top, tokens, logprobs, entropy, top_ids, top_logprobs)
-    assert logits.dtype == torch.float32 and (V == 1 or logits.stride(1) == 1)
+def token_scores(logits: torch.Tensor, vocab: int, tokens: torch.Tensor, top: int, out) -> None:
+    """Per row of ``logits`` [rows, >= vocab] (float32, a row's values side by side): the log
+    probability of ``tokens[row]`` (int32; NaN where that is no id below ``vocab``), the entropy, and
+    the ids and log probabilities of the ``top`` greatest logits, the lowest id first among equals,
+    into ``out``, a ``sampling.Scores`` of that many rows and alternatives (``token_scores`` there is
+    what checks all this)."""
     _call("scores", "mb_token_scores",
           [_vp, _ll, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp],
-          _ptr(logits), logits.stride(0), rows, V, _ptr(tokens), top, _ptr(logprobs),
-          _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs), _sms(), _stream())
-
-
-def _score_outputs(rows: int, top: int, tokens: torch.Tensor, logprobs: torch.Tensor,
-                   entropy: torch.Tensor, top_ids: torch.Tensor, top_logprobs: torch.Tensor) -> None:
-    """Contiguous lists of the sizes that the scores' kernels write (and the tokens they read)."""
-    for t, dtype, n in ((tokens, torch.int32, rows), (logprobs, torch.float32, rows),
-                        (entropy, torch.float32, rows), (top_ids, torch.int32, rows * top),
-                        (top_logprobs, torch.float32, rows * top)):
-        if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
-            raise KernelError(f"scores of {rows} rows with {top} alternatives: {t.dtype} "
-                              f"{tuple(t.shape)}, not {n} contiguous values of {dtype}")
+          logits.data_ptr(), logits.stride(0), logits.shape[0], vocab, tokens.data_ptr(), top,
+          out.logprobs.data_ptr(), out.entropy.data_ptr(), out.top_ids.data_ptr(),
+          out.top_logprobs.data_ptr(), _sms(), _stream())
 
 
 def head_scores_supported(h: torch.Tensor, w: torch.Tensor) -> bool:
@@ -1534,41 +1529,35 @@ def head_scores_supported(h: torch.Tensor, w: torch.Tensor) -> bool:
 
 
 def head_scores(h: torch.Tensor, w: torch.Tensor, limit: int, scale: float, cap: float,
-                tokens: torch.Tensor, top: int, logprobs: torch.Tensor, entropy: torch.Tensor,
-                top_ids: torch.Tensor, top_logprobs: torch.Tensor, error: torch.Tensor) -> None:
+                tokens: torch.Tensor, top: int, out, error: torch.Tensor) -> None:
     """``token_scores`` of the logits scale * h · wᵀ (of the first ``limit`` rows of ``w``; with ``cap``
     > 0: cap tanh(x / cap)) for bfloat16 h [rows, K] and w [V, K], without storing them."""
     rows, Kd = h.shape
     assert w.shape[1] == Kd and h.stride(1) == 1 and 0 < limit <= w.shape[0]
     _contig(w, "the weight")
-    _score_outputs(rows, top, tokens, logprobs, entropy, top_ids, top_logprobs)
     f, _ = _functions.get("mb_head_scores_scratch") or _function(
         "head_scores", "mb_head_scores_scratch", [_i, _i, _i, _i], _ll)
     scratch = torch.empty(f(rows, limit, top, _sms()), dtype=torch.uint8, device=h.device)
     _call("head_scores", "mb_head_scores",
           [_vp, _i, _vp, _i, _i, _i, _f, _f, _vp, _i, _vp, _vp, _vp, _vp, _vp, _ll, _vp, _i, _vp],
           _ptr(h), h.stride(0), _ptr(w), rows, limit, Kd, float(scale), float(cap), _ptr(tokens),
-          top, _ptr(logprobs), _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs), _ptr(scratch),
-          scratch.numel(), _ptr(error), _sms(), _stream(), launches=2 * -(-rows // 16384))
+          top, _ptr(out.logprobs), _ptr(out.entropy), _ptr(out.top_ids), _ptr(out.top_logprobs),
+          _ptr(scratch), scratch.numel(), _ptr(error), _sms(), _stream(),
+          launches=2 * -(-rows // 16384))
 
 
 # ------------------------------------------------------------------------------ a step's arrays
-def _lists(what: str, names: str, *tensors: torch.Tensor) -> int:
-    """The length of int32 lists, which has to be the same for all of them, as has their device."""
-    n, device = tensors[0].numel(), tensors[0].get_device()
-    for t in tensors:
-        if (t.dtype is not torch.int32 or t.numel() != n or t.dim() != 1 or not t.is_contiguous()
-                or t.get_device() != device):
-            name = names.split()[[u is t for u in tensors].index(True)]
-            raise KernelError(f"{what}: {name} is {t.dtype} {tuple(t.shape)} on {t.device}, not a "
-                              f"contiguous int32 list of {n} beside the others")
-    return n
+def _not_a_list(what: str, t: torch.Tensor, n: int) -> KernelError:
+    return KernelError(f"{what}: {t.dtype} {tuple(t.shape)} on {t.device}, not a contiguous int32 list of "
+                       f"{n} beside the others")
 
 
-def _beside(what: str, first: torch.Tensor, *others: torch.Tensor) -> None:
-    for t in others:
-        if t.get_device() != first.get_device():
-            raise KernelError(f"{what}: tensors on {first.device} and on {t.device}")
+def _is_list(t: torch.Tensor, n: int, device: int) -> bool:
+    return (t.dtype is _int32 and t.numel() == n and t.dim() == 1 and t.get_device() == device
+            and t.is_contiguous())
+
+
+_int32 = torch.int32
 
 
 def step_index(slots: torch.Tensor, past: torch.Tensor, new: torch.Tensor, seq_start: torch.Tensor,
@@ -1578,15 +1567,17 @@ def step_index(slots: torch.Tensor, past: torch.Tensor, new: torch.Tensor, seq_s
     rows and the end; per token its sequence, position and slot. The token arrays may be longer than
     the step (what lies behind it is left) or shorter (what does not fit is not written). All
     int32, on the device; nothing is read on the host."""
-    B = _lists("step_index", "slots past new", slots, past, new)
-    T = _lists("step_index", "tok_seq tok_pos tok_slot", tok_seq, tok_pos, tok_slot)
-    if _lists("step_index", "seq_start", seq_start) != B + 1:
-        raise KernelError(f"step_index: seq_start holds {seq_start.numel()} rows, not {B} + 1")
-    _beside("step_index", slots, seq_start, tok_seq)
-    with on_device_of(slots):
-        _call("step_index", "mb_step_index", [_vp, _vp, _vp, _i, _ll, _vp, _vp, _vp, _vp, _vp],
-              _ptr(slots), _ptr(past), _ptr(new), B, T, _ptr(seq_start), _ptr(tok_seq),
-              _ptr(tok_pos), _ptr(tok_slot), _stream())
+    B, T, device = slots.numel(), tok_seq.numel(), slots.get_device()
+    for t, n in ((slots, B), (past, B), (new, B), (seq_start, B + 1), (tok_seq, T), (tok_pos, T),
+                 (tok_slot, T)):
+        if not _is_list(t, n, device):
+            raise _not_a_list("step_index", t, n)
+    if elsewhere(device):
+        with on_device_of(slots):
+            return step_index(slots, past, new, seq_start, tok_seq, tok_pos, tok_slot)
+    _call("step_index", "mb_step_index", [_vp, _vp, _vp, _i, _ll, _vp, _vp, _vp, _vp, _vp],
+          slots.data_ptr(), past.data_ptr(), new.data_ptr(), B, T, seq_start.data_ptr(),
+          tok_seq.data_ptr(), tok_pos.data_ptr(), tok_slot.data_ptr(), _stream())
 
 
 def map_pages(table: torch.Tensor, slots: torch.Tensor, past: torch.Tensor, new: torch.Tensor,
@@ -1596,19 +1587,24 @@ def map_pages(table: torch.Tensor, slots: torch.Tensor, past: torch.Tensor, new:
     ``past[b] + new[b]`` positions take (at most ``ring_pages``, where that is above 0), sequence
     after sequence. Distinct slots. Entries outside the table are left, and so are those that ``pages``
     is too short for. All int32, on the device; nothing is read on the host."""
-    B = _lists("map_pages", "slots past new held", slots, past, new, held)
-    N = _lists("map_pages", "pages", pages)
-    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
-        raise KernelError(f"map_pages: the table is {table.dtype} {tuple(table.shape)}, not a "
-                          "contiguous int32 matrix")
+    B, N, device = slots.numel(), pages.numel(), slots.get_device()
+    for t, n in ((slots, B), (past, B), (new, B), (held, B), (pages, N)):
+        if not _is_list(t, n, device):
+            raise _not_a_list("map_pages", t, n)
+    if (table.dtype is not _int32 or table.dim() != 2 or not table.is_contiguous()
+            or table.get_device() != device):
+        raise KernelError(f"map_pages: the table is {table.dtype} {tuple(table.shape)} on "
+                          f"{table.device}, not a contiguous int32 matrix beside the lists")
     if ring_pages < 0:
         raise KernelError(f"map_pages: a ring of {ring_pages} pages")
-    _beside("map_pages", slots, table, pages)
-    with on_device_of(slots):
-        _call("step_index", "mb_map_pages",
-              [_vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _vp],
-              _ptr(table), table.shape[0], table.shape[1], _ptr(slots), _ptr(past), _ptr(new),
-              _ptr(held), B, _ptr(pages), N, ring_pages, _stream())
+    if elsewhere(device):
+        with on_device_of(slots):
+            return map_pages(table, slots, past, new, held, pages, ring_pages)
+    n_slots, max_pages = table.shape
+    _call("step_index", "mb_map_pages",
+          [_vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _vp],
+          table.data_ptr(), n_slots, max_pages, slots.data_ptr(), past.data_ptr(), new.data_ptr(),
+          held.data_ptr(), B, pages.data_ptr(), N, ring_pages, _stream())
 
 
 # ------------------------------------------------------------------------------ tensor cores

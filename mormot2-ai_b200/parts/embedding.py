@@ -90,7 +90,7 @@ class LmHead(Part):
             if (self.linear.fast is not None and rows > SCORE_STORED
                     and K.head_scores_supported(h, weight)):
                 K.head_scores(h, weight, limit, self.scale, self.softcap, tokens.contiguous(), top,
-                              *out.tensors(), rt.error_word)
+                              out, rt.error_word)
                 return out
             for a in range(0, rows, SCORE_BAND):
                 b = min(rows, a + SCORE_BAND)

@@ -4,6 +4,7 @@ the model's own, of the whole vocabulary: no temperature and no filter is in the
 returns chosen tokens only; scores are this library's own."""
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 from typing import List, Optional, Tuple
 
@@ -11,6 +12,13 @@ import torch
 
 from .. import kernels as K
 from ..errors import InferError
+
+
+@functools.lru_cache(maxsize=64)
+def _nothing(rows: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
+    """No alternatives' ids and log probabilities: tensors without a value."""
+    return (torch.empty((rows, 0), dtype=torch.int32, device=device),
+            torch.empty((rows, 0), dtype=torch.float32, device=device))
 
 
 @dataclass
@@ -42,8 +50,10 @@ class Scores:
     def beside(cls, tokens: torch.Tensor, rows: int, top: int) -> "Scores":
         """Scores on the device of ``tokens`` (int32)."""
         logprobs = tokens.new_empty(rows, dtype=torch.float32)
-        return cls(logprobs, logprobs.new_empty(rows), tokens.new_empty((rows, top)),
-                   logprobs.new_empty((rows, top)))
+        entropy = logprobs.new_empty(rows)
+        if top == 0:
+            return cls(logprobs, entropy, *_nothing(rows, tokens.device))
+        return cls(logprobs, entropy, tokens.new_empty((rows, top)), logprobs.new_empty((rows, top)))
 
     @classmethod
     def packed(cls, buffer: torch.Tensor, rows: int, top: int) -> "Scores":
@@ -100,6 +110,15 @@ def check_tokens(tokens: torch.Tensor, rows: int, device: int) -> None:
                          f"{tokens.device}, not int32 [{rows}] beside them")
 
 
+def check_out(out: Scores, rows: int, top: int, device: int) -> None:
+    for t, dtype, shape in zip(out.tensors(), (torch.float32, torch.float32, torch.int32, torch.float32),
+                               ((rows,), (rows,), (rows, top), (rows, top))):
+        if (t.dtype is not dtype or t.shape != shape or not t.is_contiguous()
+                or t.get_device() != device):
+            raise InferError(f"scores of {rows} rows and {top} alternatives into {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
+
+
 def check_score(h: torch.Tensor, tokens: torch.Tensor, top: int, hidden: int, vocab: int,
                 vocab_limit: Optional[int]) -> int:
     """Refuses what a head of ``vocab`` rows of ``hidden`` values cannot score; how many ids take
@@ -120,26 +139,28 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     ``top``: alternatives, up to 32. ``vocab_limit``: only the ids below it take part. ``out``: to
     write into, contiguous, as ``Scores.empty`` makes it. Runs on the current stream of the logits'
     device and reads nothing back; what it needs besides is allocated for the call alone."""
-    if logits.dim() != 2 or logits.dtype is not torch.float32 or logits.shape[1] == 0:
-        raise InferError(f"scores: logits are {logits.dtype} {tuple(logits.shape)}, not float32 "
-                         "[rows, vocab]")
-    rows, vocab = logits.shape
+    shape = logits.shape
+    if len(shape) != 2 or logits.dtype is not torch.float32 or shape[1] == 0:
+        raise InferError(f"scores: logits are {logits.dtype} {tuple(shape)}, not float32 [rows, vocab]")
+    rows, vocab = shape
     if vocab > 1 and logits.stride(1) != 1:
         raise InferError("scores: the logits of a row do not lie side by side")
     if vocab_limit is not None:
         vocab = candidates(vocab, vocab_limit)
-        logits = logits[:, :vocab]
     check_top(top, vocab)
-    check_tokens(tokens, rows, logits.get_device())
+    device = logits.get_device()
+    check_tokens(tokens, rows, device)
     if out is None:
         out = Scores.beside(tokens, rows, top)
-    elif (out.top_ids.shape != (rows, top) or out.logprobs.get_device() != tokens.get_device()):
-        raise InferError(f"scores of {rows} rows and {top} alternatives into {tuple(out.top_ids.shape)} "
-                         f"on {out.logprobs.device}")
+    else:
+        check_out(out, rows, top, device)
     if rows == 0:
         return out
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
-    with K.on_device_of(logits):
-        K.token_scores(logits, tokens, top, out.logprobs, out.entropy, out.top_ids, out.top_logprobs)
+    if K.elsewhere(device):
+        with K.on_device_of(logits):
+            K.token_scores(logits, vocab, tokens, top, out)
+    else:
+        K.token_scores(logits, vocab, tokens, top, out)
     return out
