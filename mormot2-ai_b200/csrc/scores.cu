@@ -22,8 +22,8 @@ __device__ __forceinline__ uint32_t sc_at_leader(const void* p) {     // this sh
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(0));
   return r;
 }
-__device__ __forceinline__ void sc_put(uint32_t at, TopKey v) {
-  asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
+__device__ __forceinline__ void sc_put(uint32_t at, uint32_t v) {
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 __device__ __forceinline__ void sc_put(uint32_t at, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
@@ -59,7 +59,8 @@ struct ScShared {
   Mass part[SC_WARPS];
   // of the cluster's first CTA: every CTA's part
   Mass mass[SC_CLUSTER];
-  TopKey keys[SC_CLUSTER][MB_SCORES_TOP];
+  alignas(16) uint32_t all_place[SC_CLUSTER * MB_SCORES_TOP];
+  uint32_t all_id[SC_CLUSTER * MB_SCORES_TOP];
 };
 
 // Values `base` .. of the row's part x[0 .. n): value 4 i + j of a thread is at `place`
@@ -101,15 +102,16 @@ __device__ __forceinline__ int sc_above(const uint32_t* list, int n, uint32_t p)
   return above;
 }
 
-// The `top` greatest of the `n` keys in sh.place and sh.id, in order into sh.sorted: a key's place is the
-// number of keys above it, for which its value alone is looked at unless two are equal. `turn` counts
-// these calls (sh.taken and sh.equal[turn & 1] are 0 before each).
-__device__ __forceinline__ void sc_sort(int n, int top, int turn, ScShared& sh) {
+// The `top` greatest of `n` keys, in order into sh.sorted: a key's place is the number of keys above it,
+// for which its value alone is looked at unless two are equal. `turn` counts these calls (sh.taken and
+// sh.equal[turn & 1] are 0 before each).
+__device__ __forceinline__ void sc_sort(const uint32_t* place, const uint32_t* id, int n, int top, int turn,
+                                        ScShared& sh) {
   for (int i = threadIdx.x; i < n; i += SC_THREADS) {
-    const uint32_t p = sh.place[i];
-    const int above = sc_above(sh.place, n, p);
+    const uint32_t p = place[i];
+    const int above = sc_above(place, n, p);
     if (above < top) {
-      sh.sorted[above] = (TopKey)p << 32 | sh.id[i];
+      sh.sorted[above] = (TopKey)p << 32 | id[i];
       if (atomicAdd(&sh.taken[above], 1) > 0) sh.equal[turn & 1] = 1;
     }
   }
@@ -119,9 +121,9 @@ __device__ __forceinline__ void sc_sort(int n, int top, int turn, ScShared& sh) 
   if (threadIdx.x == 0) sh.equal[(turn + 1) & 1] = 0;
   if (!equal) return;
   for (int i = threadIdx.x; i < n; i += SC_THREADS) {
-    const TopKey k = (TopKey)sh.place[i] << 32 | sh.id[i];
+    const TopKey k = (TopKey)place[i] << 32 | id[i];
     int above = 0;
-    for (int j = 0; j < n; ++j) above += ((TopKey)sh.place[j] << 32 | sh.id[j]) > k;
+    for (int j = 0; j < n; ++j) above += ((TopKey)place[j] << 32 | id[j]) > k;
     if (above < top) sh.sorted[above] = k;
   }
   __syncthreads();
@@ -165,12 +167,12 @@ __device__ __noinline__ void sc_pick(const float* __restrict__ x, int base, int 
 // the bar is the `top`-th greatest value so far, which hardly any value passes, and a round costs what the
 // sums cost, and one barrier. Each thread's sums are over the greatest value that it has seen itself.
 template <int EACH, bool WIDE, bool TOP>
-__device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int id0, int top, ScShared& sh) {
+__device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int id0, int top, int& turn, ScShared& sh) {
   constexpr int ROUND = SC_THREADS * EACH;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Mass mine = mass_none();
   float bar = -3.402823466e38f;        // the lowest finite value: -infinity and NaN never pass
-  int held = 0, turn = 0, third = 0;   // keys in sh.sorted; sorts; the round's counter of three
+  int held = 0, third = 0;             // keys in sh.sorted; the round's counter of three
   if (TOP) {
     if (threadIdx.x < MB_SCORES_TOP) sh.taken[threadIdx.x] = 0;
     if (threadIdx.x == 0) sh.passed[0] = sh.n_heads = sh.equal[0] = 0, sh.least = ~0u;
@@ -225,7 +227,7 @@ __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int 
     third = next;
     if (passed == 0) continue;
     if (held + passed <= SC_ROOM) {
-      sc_sort(held + passed, top, turn++, sh);
+      sc_sort(sh.place, sh.id, held + passed, top, turn++, sh);
       held = min(top, held + passed);
     } else {
       sc_pick(x, base, min(n, base + ROUND), id0, held, top, sh);
@@ -262,7 +264,9 @@ token_scores_kernel(const float* __restrict__ logits, size_t stride, int V, int 
   }
   const int i0 = part * per, n = max(0, min(per, V - i0));
   const bool wide = ((uintptr_t)x & 15) == 0;
-  const Mass v = wide ? sc_part<EACH, true, TOP>(x + i0, n, i0, top, sh) : sc_part<EACH, false, TOP>(x + i0, n, i0, top, sh);
+  int turn = 0;
+  const Mass v = wide ? sc_part<EACH, true, TOP>(x + i0, n, i0, top, turn, sh)
+                      : sc_part<EACH, false, TOP>(x + i0, n, i0, top, turn, sh);
   if (parts > 1) {
     sc_wait();
     if (threadIdx.x == 0) {
@@ -270,13 +274,21 @@ token_scores_kernel(const float* __restrict__ logits, size_t stride, int V, int 
       sc_put(sc_at_leader(&sh.mass[part].s), v.s);
       sc_put(sc_at_leader(&sh.mass[part].t), v.t);
     }
-    if (TOP && threadIdx.x < top) sc_put(sc_at_leader(&sh.keys[part][threadIdx.x]), sh.sorted[threadIdx.x]);
+    if (TOP && threadIdx.x < top) {
+      const TopKey k = sh.sorted[threadIdx.x];
+      sc_put(sc_at_leader(&sh.all_place[part * top + threadIdx.x]), (uint32_t)(k >> 32));
+      sc_put(sc_at_leader(&sh.all_id[part * top + threadIdx.x]), (uint32_t)k);
+    }
     sc_arrive();
     sc_wait();
     if (part > 0) return;
+    if (TOP) {
+      if (threadIdx.x < top) sh.sorted[threadIdx.x] = 0;      // there may be fewer keys
+      __syncthreads();
+      sc_sort(sh.all_place, sh.all_id, parts * top, top, turn, sh);
+    }
   } else {
     if (threadIdx.x == 0) sh.mass[0] = v;
-    if (TOP && threadIdx.x < top) sh.keys[0][threadIdx.x] = sh.sorted[threadIdx.x];
     __syncthreads();
   }
   if (threadIdx.x >= 32) return;
@@ -286,22 +298,7 @@ token_scores_kernel(const float* __restrict__ logits, size_t stride, int V, int 
   for (int o = SC_CLUSTER / 2; o > 0; o >>= 1)
     all = mass_join(all, {__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.s, o),
                           __shfl_xor_sync(0xffffffffu, all.t, o)});
-  TopKey mine = 0;
-  if (TOP) {      // every part's keys are in order: the greatest of their heads, `top` times
-    int head = 0;
-    for (int j = 0; j < top; ++j) {
-      const TopKey k = lane < parts && head < top ? sh.keys[lane][head] : 0;
-      TopKey best = k;
-#pragma unroll
-      for (int o = SC_CLUSTER / 2; o > 0; o >>= 1) {
-        const TopKey c = __shfl_xor_sync(0xffffffffu, best, o);
-        if (c > best) best = c;
-      }
-      best = __shfl_sync(0xffffffffu, best, 0);
-      if (k == best) ++head;
-      if (lane == j) mine = best;
-    }
-  }
+  const TopKey mine = TOP && lane < top ? sh.sorted[lane] : 0;
   all = {__shfl_sync(0xffffffffu, all.m, 0), __shfl_sync(0xffffffffu, all.s, 0), __shfl_sync(0xffffffffu, all.t, 0)};
   finish_row(all, __shfl_sync(0xffffffffu, given, 0), mine, top, row, out);
 }

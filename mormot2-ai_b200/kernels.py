@@ -1552,11 +1552,6 @@ def _not_a_list(what: str, t: torch.Tensor, n: int) -> KernelError:
                        f"{n} beside the others")
 
 
-def _is_list(t: torch.Tensor, n: int, device: int) -> bool:
-    return (t.dtype is _int32 and t.numel() == n and t.dim() == 1 and t.get_device() == device
-            and t.is_contiguous())
-
-
 _int32 = torch.int32
 
 
@@ -1570,7 +1565,8 @@ def step_index(slots: torch.Tensor, past: torch.Tensor, new: torch.Tensor, seq_s
     B, T, device = slots.numel(), tok_seq.numel(), slots.get_device()
     for t, n in ((slots, B), (past, B), (new, B), (seq_start, B + 1), (tok_seq, T), (tok_pos, T),
                  (tok_slot, T)):
-        if not _is_list(t, n, device):
+        if (t.dtype is not _int32 or t.numel() != n or t.dim() != 1 or t.get_device() != device
+                or not t.is_contiguous()):
             raise _not_a_list("step_index", t, n)
     if elsewhere(device):
         with on_device_of(slots):
@@ -1589,7 +1585,8 @@ def map_pages(table: torch.Tensor, slots: torch.Tensor, past: torch.Tensor, new:
     is too short for. All int32, on the device; nothing is read on the host."""
     B, N, device = slots.numel(), pages.numel(), slots.get_device()
     for t, n in ((slots, B), (past, B), (new, B), (held, B), (pages, N)):
-        if not _is_list(t, n, device):
+        if (t.dtype is not _int32 or t.numel() != n or t.dim() != 1 or t.get_device() != device
+                or not t.is_contiguous()):
             raise _not_a_list("map_pages", t, n)
     if (table.dtype is not _int32 or table.dim() != 2 or not table.is_contiguous()
             or table.get_device() != device):

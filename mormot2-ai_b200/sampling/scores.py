@@ -44,16 +44,16 @@ class Scores:
 
     @classmethod
     def empty(cls, rows: int, top: int, device) -> "Scores":
-        return cls.beside(torch.empty(rows, dtype=torch.int32, device=device), rows, top)
+        return cls.beside(torch.empty(rows, dtype=torch.float32, device=device),
+                          torch.empty(0, dtype=torch.int32, device=device), rows, top)
 
     @classmethod
-    def beside(cls, tokens: torch.Tensor, rows: int, top: int) -> "Scores":
-        """Scores on the device of ``tokens`` (int32)."""
-        logprobs = tokens.new_empty(rows, dtype=torch.float32)
-        entropy = logprobs.new_empty(rows)
+    def beside(cls, floats: torch.Tensor, ints: torch.Tensor, rows: int, top: int) -> "Scores":
+        """Scores on the device of a float32 and an int32 tensor."""
+        logprobs, entropy = floats.new_empty(rows), floats.new_empty(rows)
         if top == 0:
-            return cls(logprobs, entropy, *_nothing(rows, tokens.device))
-        return cls(logprobs, entropy, tokens.new_empty((rows, top)), logprobs.new_empty((rows, top)))
+            return cls(logprobs, entropy, *_nothing(rows, ints.device))
+        return cls(logprobs, entropy, ints.new_empty((rows, top)), floats.new_empty((rows, top)))
 
     @classmethod
     def packed(cls, buffer: torch.Tensor, rows: int, top: int) -> "Scores":
@@ -151,7 +151,7 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     device = logits.get_device()
     check_tokens(tokens, rows, device)
     if out is None:
-        out = Scores.beside(tokens, rows, top)
+        out = Scores.beside(logits, tokens, rows, top)
     else:
         check_out(out, rows, top, device)
     if rows == 0:
