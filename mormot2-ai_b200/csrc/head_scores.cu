@@ -62,14 +62,27 @@ struct HeadWalk {
 template <int N> struct TopList {
   float v[N];
   int id[N];
+  float bar;      // what a value has to pass
   __device__ __forceinline__ void clear(int top) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       v[i] = i < N - top ? INFINITY : -INFINITY;
       id[i] = -1;
     }
+    bar = -INFINITY;
   }
-  __device__ __forceinline__ float bar() const { return v[N - 1]; }
+  // One of many groups' greatest values: in the end the least of v is below no more than top - 1 groups
+  __device__ __forceinline__ void probe(float x) {
+#pragma unroll
+    for (int k = N - 1; k > 0; --k) v[k] = fmaxf(v[k], fminf(v[k - 1], x));
+    v[0] = fmaxf(v[0], x);
+  }
+  // The list anew, with a bar a little below that value: at least `top` values pass it
+  __device__ __forceinline__ void start(int top) {
+    const float least = v[N - 1];
+    clear(top);
+    if (least > -INFINITY) bar = least - 1e-6f * fabsf(least) - 1e-30f;
+  }
   __device__ __forceinline__ void offer(float x, int i) {
     bool past[N];
 #pragma unroll
@@ -81,6 +94,7 @@ template <int N> struct TopList {
     }
     v[0] = past[0] ? x : v[0];
     id[0] = past[0] ? i : id[0];
+    bar = fmaxf(bar, v[N - 1]);
   }
   __device__ __forceinline__ void write(TopKey* keys, int top) const {
 #pragma unroll
@@ -89,8 +103,10 @@ template <int N> struct TopList {
   }
 };
 template <> struct TopList<0> {
+  static constexpr float bar = 0.f;
   __device__ __forceinline__ void clear(int) {}
-  __device__ __forceinline__ float bar() const { return 0.f; }
+  __device__ __forceinline__ void probe(float) {}
+  __device__ __forceinline__ void start(int) {}
   __device__ __forceinline__ void offer(float, int) {}
   __device__ __forceinline__ void write(TopKey*, int) const {}
 };
@@ -242,16 +258,37 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       float m = -INFINITY, s = 0.f, t = 0.f;     // the row's mass
       TopList<N> list;
       list.clear(top);
+      bool fresh = true;
       const bool idle = walk.row0() + (int)rank * 128 + q * 32 >= rows;    // none of the warp's rows is there
       for (; walk.n < walk.end; walk.step(), ++it) {
         const int b = it & 1, cols = walk.cols();
         mbar_wait(acc_full0 + 8 * b, (it >> 1) & 1, error, 64);
         tc_fence_after_sync();
         float tile_s = 0.f, tile_t = 0.f;        // the tile's part, over the same maximum
+        const uint32_t taddr = tmem + b * 256 + ((uint32_t)(q * 32) << 16);
+        if (N > 0 && fresh && !idle) {
+          // A strip's first tile is read ahead for a bar: the `top`-th of its eights' greatest values. Without
+          // it the first values of all rows pass, one after another.
+          fresh = false;
+#pragma unroll 1
+          for (int c = 0; c < cols; c += 32) {
+            float x[32];
+            load32(taddr + c, x);
+            if (shaped) shape32(x, scale, cap);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              float m = x[8 * g];
+#pragma unroll
+              for (int j = 1; j < 8; ++j) m = fmaxf(m, x[8 * g + j]);
+              if (c + 8 * g + 8 <= cols) list.probe(m);
+            }
+          }
+          list.start(top);
+        }
 #pragma unroll 1
         for (int c = 0; c < (idle ? 0 : cols); c += 32) {
           float x[32];
-          load32(tmem + b * 256 + ((uint32_t)(q * 32) << 16) + c, x);
+          load32(taddr + c, x);
           const int n = min(32, cols - c), id0 = walk.n + c;
           if (shaped) shape32(x, scale, cap);
           if (n < 32) {
@@ -274,14 +311,14 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             for (int j = 0; j < 32; ++j)
               if (off == (unsigned)j && j < n) given[row] = x[j];
           }
-          if (N > 0 && __any_sync(0xffffffffu, most > list.bar())) {
+          if (N > 0 && __any_sync(0xffffffffu, most > list.bar)) {
             // Which values pass is a bit each; a lane takes its own one after another. They are read
             // again from shared memory, where a register could not be named by a number.
             unsigned pass = 0;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + j * 128), "f"(x[j]) : "memory");
-              if (x[j] > list.bar()) pass |= 1u << j;
+              if (x[j] > list.bar) pass |= 1u << j;
             }
             while (pass) {
               const int j = __ffs(pass) - 1;
@@ -375,14 +412,16 @@ head_join_kernel(const __grid_constant__ HeadPlan plan, const Mass* __restrict__
 typedef void (*HeadKernel)(CUtensorMap, CUtensorMap, HeadPlan, int, int, int, float, float, const int*, int,
                            float*, Mass*, TopKey*, int*);
 // The kernel whose lists have room for `top` keys
-static int head_form(int top) { return (top + 7) / 8; }
+#define HS_FORMS 9
+static int head_form(int top) { return (top + 3) / 4; }
 static HeadKernel head_kernel(int form) {
-  static const HeadKernel kernels[5] = {head_scores_kernel<0>, head_scores_kernel<8>, head_scores_kernel<16>,
-                                        head_scores_kernel<24>, head_scores_kernel<32>};
+  static const HeadKernel kernels[HS_FORMS] = {
+      head_scores_kernel<0>,  head_scores_kernel<4>,  head_scores_kernel<8>,  head_scores_kernel<12>, head_scores_kernel<16>,
+      head_scores_kernel<20>, head_scores_kernel<24>, head_scores_kernel<28>, head_scores_kernel<32>};
   return kernels[form];
 }
 static cudaError_t allow_smem(int form) {
-  static unsigned long long done[5] = {0, 0, 0, 0, 0};
+  static unsigned long long done[HS_FORMS] = {};
   return mb_allow_smem((const void*)head_kernel(form), HS_SMEM, &done[form]);
 }
 
@@ -390,7 +429,7 @@ static cudaError_t allow_smem(int form) {
 static int head_pairs(int sms) {
   static int pairs = -1;
   if (pairs >= 0) return pairs;
-  if (allow_smem(4) != cudaSuccess) {
+  if (allow_smem(HS_FORMS - 1) != cudaSuccess) {
     cudaGetLastError();
     return pairs = 0;
   }
@@ -406,7 +445,7 @@ static int head_pairs(int sms) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, head_kernel(4), &cfg) != cudaSuccess) {
+  if (cudaOccupancyMaxActiveClusters(&n, head_kernel(HS_FORMS - 1), &cfg) != cudaSuccess) {
     cudaGetLastError();
     n = 0;
   }
