@@ -169,46 +169,58 @@ class CacheBook:
         ``requests = [(slot, new_length)]``. All or nothing: if a pool runs out, nothing is
         mapped and ``CacheError`` is raised. Returns, per group, the new table entries
         ``(slot, entry, page)``."""
-        out = []
-        for held, pages in self.grow(requests):
-            entries, at = [], 0
+        out: List[List[Tuple[int, int, int]]] = [[] for _ in self.plans]
+        longest: Dict[int, int] = {}            # a slot may be named twice
+        for slot, new_length in requests:
+            longest[slot] = max(longest.get(slot, 0), new_length)
+        requests = list(longest.items())
+        for g, (held, pages) in enumerate(self.grow(requests)):
+            at = 0
             for (slot, _), (h, n) in zip(requests, held):
-                entries += [(slot, h + j, page) for j, page in enumerate(pages[at:at + n])]
+                out[g] += [(slot, h + j, page) for j, page in enumerate(pages[at:at + n])]
                 at += n
-            out.append(entries)
         return out
 
     def grow(self, requests: List[Tuple[int, int]]) -> List[Tuple[List[Tuple[int, int]], List[int]]]:
-        """``reserve`` that names no entry by itself: per group ``(held, pages)``, for every request
-        the pages that its slot held before and how many it received, and all received pages in that
-        order."""
+        """``reserve`` of distinct slots that names no entry by itself: per group ``(held, pages)``,
+        for every request the pages that its slot held before and how many it received, and all
+        received pages in that order."""
         for slot, new_length in requests:
             self.check_open(slot)
             if new_length > self.max_context:
                 raise CacheError(
                     f"slot {slot}: {new_length} positions exceed the context of {self.max_context}")
+        every = []                 # per group, what every slot holds and still needs
         for g, pool in enumerate(self.pools):
-            want = 0
+            ring, mine = self.plans[g].ring_pages, self.pages[g]
+            held, want = [], 0
             for slot, new_length in requests:
-                want += max(0, self.entries_needed(g, new_length) - len(self.pages[g][slot]))
+                have = len(mine[slot])
+                n = (new_length + PAGE - 1) // PAGE
+                if ring and n > ring:
+                    n = ring
+                n = n - have if n > have else 0
+                held.append((have, n))
+                want += n
             if want > pool.free:
                 raise CacheError(
                     f"the cache is full: {want} more pages needed, {pool.free} of "
                     f"{pool.count} free")
+            every.append((held, want))
         out = []
         for g, pool in enumerate(self.pools):
-            held, pages = [], []
-            for slot, new_length in requests:
-                mine = self.pages[g][slot]
-                n = max(0, self.entries_needed(g, new_length) - len(mine))
-                held.append((len(mine), n))
+            held, want = every[g]
+            pages = pool.take_many(want)
+            at = 0
+            for (slot, _), (_, n) in zip(requests, held):
                 if n:
-                    got = pool.take_many(n)
-                    mine += got
-                    pages += got
+                    self.pages[g][slot] += pages[at:at + n]
+                    at += n
             out.append((held, pages))
+        high = self.high
         for slot, new_length in requests:
-            self.high[slot] = max(self.high[slot], new_length)
+            if new_length > high[slot]:
+                high[slot] = new_length
         return out
 
     def commit(self, slot: int, new_length: int) -> None:

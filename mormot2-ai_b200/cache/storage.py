@@ -11,15 +11,11 @@ from __future__ import annotations
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Tuple
 
-import numpy as np
 import torch
 
 from .. import kernels as K
 from .guards import Guards, alloc
 from .pages import PAGE, CacheBook, GroupPlan
-
-# Entries of a page table that are copied as whole rows; more are written by a kernel.
-MAP_ROWS = 8192
 
 
 @dataclass
@@ -43,7 +39,6 @@ class CacheStorage:
         self.plans = plans
         self.pools: List[torch.Tensor] = []
         self.tables: List[torch.Tensor] = []
-        self.tables_host: List[torch.Tensor] = []
         self.lines: Dict[int, CacheLine] = {}
         self.value_pools: Dict[int, torch.Tensor] = {}   # of groups whose value rows differ in size
         for g, plan in enumerate(plans):
@@ -63,12 +58,8 @@ class CacheStorage:
                              dtype, device)
             table = alloc(guards, f"page table of group {g}", (max_slots, plan.max_pages),
                           torch.int32, device)
-            # pageable on purpose: the copy to the device then reads it before returning, so the
-            # host may change it again at once
-            host = torch.zeros((max_slots, plan.max_pages), dtype=torch.int32)
             self.pools.append(pool)
             self.tables.append(table)
-            self.tables_host.append(host)
             for i, line in enumerate(plan.lines):
                 if g in self.value_pools:
                     values = self.value_pools[g][i]
@@ -77,6 +68,12 @@ class CacheStorage:
                 self.lines[line] = CacheLine(pool[i, 0], values, table, plan.max_pages,
                                              plan.ring_pages, plan.window, plan.kv_heads,
                                              plan.head_dim, v_dim)
+        # what a step's new pages are written to the tables from: per group five lists at most
+        room = sum(4 * max_slots + p.n_pages for p in plans)
+        self.lists_host = torch.zeros(room, dtype=torch.int32).pin_memory() if room else None
+        self.lists = alloc(guards, "lists of new pages", (room,), torch.int32, device)
+        self.lists_copied = torch.cuda.Event()
+        self.lists_busy = False
         # fixed-size state per slot, at its initial value when a sequence starts; beside it a
         # copy of the same size that a step saves the slots it touches into, so that a step
         # that fails half way leaves the state it found
@@ -95,40 +92,62 @@ class CacheStorage:
 
     def map_pages(self, new_entries: List[List[Tuple[int, int, int]]]) -> None:
         """Writes the new table entries of ``CacheBook.reserve`` to the device tables, in the order of
-        the stream. The copy stages the host's entries before it returns; waiting for its end as
-        well would keep a step's launches from going out while the step before still runs."""
+        the stream; whatever is launched next finds them there."""
+        work = []
         for g, entries in enumerate(new_entries):
-            if not entries:
-                continue
-            host = self.tables_host[g]
-            where = np.asarray(entries, dtype=np.int64)     # [n, 3]: slot, entry, page
-            host.numpy()[where[:, 0], where[:, 1]] = where[:, 2]
-            lo, hi = int(where[:, 0].min()), int(where[:, 0].max())
-            self.tables[g][lo:hi + 1].copy_(host[lo:hi + 1], non_blocking=True)
+            first: Dict[int, int] = {}
+            many: Dict[int, int] = {}
+            for slot, entry, _ in entries:
+                first.setdefault(slot, entry)
+                many[slot] = many.get(slot, 0) + 1
+            pages = {slot: [] for slot in first}
+            for slot, _, page in entries:
+                pages[slot].append(page)
+            work.append((list(first), [0] * len(first),
+                         [PAGE * (first[s] + many[s]) for s in first], list(first.values()),
+                         [p for s in first for p in pages[s]]))
+        if self._write_entries(work):
+            # a kernel may read a table ahead of its wait for the kernel before it, which then must
+            # not be the one that wrote it
+            self.lists[:1].copy_(self.lists_host[:1], non_blocking=True)
+            self.lists_copied.record()
 
     def map_grown(self, slots: List[int], past: List[int], new: List[int], grown) -> None:
         """``map_pages`` for what ``CacheBook.grow`` returned for distinct ``slots`` that held
-        ``past`` positions and grow by ``new``. Where whole rows of the tables would be many bytes,
-        the lengths and the pages alone are copied and a kernel writes the entries."""
-        for g, (held, pages) in enumerate(grown):
-            if not pages:
+        ``past`` positions and grow by ``new``. A copy has to follow on the stream before kernels that
+        read tables ahead of their waits (the one of the step's index arrays does)."""
+        work = []
+        for held, pages in grown:
+            if len(pages) <= 0:
+                work.append(())
                 continue
-            host = self.tables_host[g].numpy()
-            at, lo, hi = 0, len(host), 0
-            for slot, (h, n) in zip(slots, held):
-                if n:
-                    host[slot, h:h + n] = pages[at:at + n]
-                    at += n
-                    lo, hi = min(lo, slot), max(hi, slot)
-            if (hi + 1 - lo) * host.shape[1] <= MAP_ROWS:
-                self.tables[g][lo:hi + 1].copy_(self.tables_host[g][lo:hi + 1], non_blocking=True)
-                continue
-            B = len(slots)
-            lists = np.array([*slots, *past, *new, *(h for h, _ in held), *pages], dtype=np.int32)
-            # (pageable: staged before the copy returns)
-            dev = torch.from_numpy(lists).to(self.tables[g].device, non_blocking=True)
-            K.map_pages(self.tables[g], dev[:B], dev[B:2 * B], dev[2 * B:3 * B], dev[3 * B:4 * B],
-                        dev[4 * B:], self.plans[g].ring_pages)
+            some = [i for i, (_, n) in enumerate(held) if n]
+            work.append(([slots[i] for i in some], [past[i] for i in some], [new[i] for i in some],
+                         [held[i][0] for i in some], pages))
+        self._write_entries(work)
+
+    def _write_entries(self, work) -> bool:
+        """Per group the slots, past and new positions, pages held, and new pages; whether there
+        were any. The lists go to the device in one copy."""
+        flat: List[int] = []
+        for lists in work:
+            for one in lists:
+                flat += one
+        if not flat:
+            return False
+        if self.lists_busy:
+            self.lists_copied.synchronize()          # the last copy must have read the host's lists
+        self.lists_host.numpy()[:len(flat)] = flat
+        self.lists[:len(flat)].copy_(self.lists_host[:len(flat)], non_blocking=True)
+        self.lists_copied.record()
+        self.lists_busy = True
+        at = 0
+        for g, lists in enumerate(work):
+            if lists and lists[0]:
+                B, N = len(lists[0]), len(lists[4])
+                K.map_pages_packed(self.tables[g], self.lists, at, B, N, self.plans[g].ring_pages)
+                at += 4 * B + N
+        return True
 
     def table_faults(self, book: CacheBook) -> List[str]:
         """Compares the page tables on the device with the bookkeeping: every entry that a

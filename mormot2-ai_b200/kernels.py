@@ -1604,6 +1604,19 @@ def map_pages(table: torch.Tensor, slots: torch.Tensor, past: torch.Tensor, new:
           held.data_ptr(), B, pages.data_ptr(), N, ring_pages, _stream())
 
 
+def map_pages_packed(table: torch.Tensor, lists: torch.Tensor, at: int, B: int, N: int,
+                     ring_pages: int) -> None:
+    """``map_pages`` of lists that lie one after another in ``lists`` from value ``at`` on: ``B``
+    slots, past, new and held, and ``N`` pages."""
+    assert lists.dtype == table.dtype == torch.int32 and at + 4 * B + N <= lists.numel()
+    p = lists.data_ptr() + 4 * at
+    n_slots, max_pages = table.shape
+    _call("step_index", "mb_map_pages",
+          [_vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _vp],
+          table.data_ptr(), n_slots, max_pages, p, p + 4 * B, p + 8 * B, p + 12 * B, B, p + 16 * B, N,
+          ring_pages, _stream())
+
+
 # ------------------------------------------------------------------------------ tensor cores
 def gemm_tc_supported(a: torch.Tensor, w: torch.Tensor) -> bool:
     lib = build.load_library("gemm_tc")

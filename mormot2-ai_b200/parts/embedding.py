@@ -10,15 +10,22 @@ from typing import Dict, List, Optional
 import torch
 
 from .. import kernels as K
-from ..sampling.scores import Scores, check_score, token_scores
+from ..sampling.scores import Scores, check_score
 from .base import EMBEDDINGS, ENTRIES, HEADS, Part, TensorNeed
 from .linear import Linear, Pending
 
 
-# bfloat16 rows up to which logits are stored and scored from there
-SCORE_STORED = 64
-# Rows whose logits are stored at a time where they are scored through memory
-SCORE_BAND = 256
+# Logits of rows whose scores go through memory: so many values at a time (1 GiB)
+SCORE_BAND = 1 << 28
+
+
+def scores_through_memory(rows: int, width: int, top: int) -> bool:
+    """Whether the logits of so few rows are better stored: the product of few rows streams the head
+    faster, while a strip of the fused kernel pays for its first tile and its lists. 151,936 ids, us
+    fused | stored, with 5 alternatives: 16 rows of 1,024 values 86 | 70, 48 rows 83 | 77, 64 rows 75 | 80,
+    32 rows of 2,048 114 | 115, 48 rows of 4,096 224 | 233; with 20: 128 rows of 512 105 | 79, of 1,024
+    111 | 109, 64 rows of 2,048 148 | 139, of 4,096 232 | 261."""
+    return rows <= 32 or rows * width <= (49152 if top <= 8 else 131072)
 
 
 class TokenEmbedding(Part):
@@ -81,20 +88,26 @@ class LmHead(Part):
         ``token_scores`` of ``forward(h)`` gives them. Of more than a few bfloat16 rows the logits are
         never stored (``csrc/head_scores.cu``); others go through memory, a band of rows at a time."""
         limit = check_score(h, tokens, top, self.hidden, self.vocab, vocab_limit)
+        if K.elsewhere(h.get_device()):
+            with K.on_device_of(h):
+                return self.score(h, tokens, top, vocab_limit)
         rows = h.shape[0]
         out = Scores.empty(rows, top, h.device)
         if rows == 0:
             return out
-        with K.on_device_of(h):
-            weight, rt = self.linear.weight, self.linear.rt
-            if (self.linear.fast is not None and rows > SCORE_STORED
-                    and K.head_scores_supported(h, weight)):
-                K.head_scores(h, weight, limit, self.scale, self.softcap, tokens.contiguous(), top,
-                              out, rt.error_word)
-                return out
-            for a in range(0, rows, SCORE_BAND):
-                b = min(rows, a + SCORE_BAND)
-                token_scores(self.forward(h[a:b]), tokens[a:b], top, vocab_limit, out.rows(a, b))
+        weight, rt = self.linear.weight, self.linear.rt
+        tokens = tokens.contiguous()
+        if (self.linear.fast is not None and not scores_through_memory(rows, self.hidden, top)
+                and K.head_scores_supported(h, weight)):
+            K.head_scores(h, weight, limit, self.scale, self.softcap, tokens, top, out, rt.error_word)
+            return out
+        band = max(256, SCORE_BAND // self.vocab)
+        if rows <= band:
+            K.token_scores(self.forward(h), limit, tokens, top, out)
+            return out
+        for a in range(0, rows, band):
+            b = min(rows, a + band)
+            K.token_scores(self.forward(h[a:b]), limit, tokens[a:b], top, out.rows(a, b))
         return out
 
 

@@ -44,8 +44,8 @@ class Scores:
 
     @classmethod
     def empty(cls, rows: int, top: int, device) -> "Scores":
-        return cls.beside(torch.empty(rows, dtype=torch.float32, device=device),
-                          torch.empty(0, dtype=torch.int32, device=device), rows, top)
+        floats = torch.empty(rows, dtype=torch.float32, device=device)
+        return cls.beside(floats, floats.view(torch.int32), rows, top)
 
     @classmethod
     def beside(cls, floats: torch.Tensor, ints: torch.Tensor, rows: int, top: int) -> "Scores":

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from mormot2_ai_b200 import InferError, PartSpec, Runtime, token_scores
-from mormot2_ai_b200.parts import HEADS
+from mormot2_ai_b200.parts import HEADS, embedding
 from mormot2_ai_b200.sampling import Scores
 from tests import score_oracle as oracle
 from tests.gpu_helpers import DEV
@@ -160,6 +160,14 @@ def test_the_same_again_on_streams_and_in_graphs():
 
 
 # ---------------------------------------------------------------------------- the head
+@pytest.fixture(params=["as it chooses", "fused"])
+def form(request, monkeypatch):
+    """The head's own choice between its forms, and the fused one for every bfloat16 row count."""
+    if request.param == "fused":
+        monkeypatch.setattr(embedding, "scores_through_memory", lambda *sizes: False)
+    return request.param
+
+
 def make_head(weight, dtype, **more):
     rt = Runtime(dtype, DEV)
     head = HEADS.build(PartSpec("lm_head", {"name": "w", "tied": False, "vocab_size": weight.shape[0],
@@ -187,7 +195,7 @@ def head_case(rows, V, K, seed, dtype):
     (1, 257, 64, 5), (1, 40000, 128, 32), (16, 1000, 96, 1), (17, 3001, 64, 0), (64, 5003, 192, 20),
     (65, 2048, 72, 7), (128, 509, 256, 32), (129, 700, 64, 5), (255, 20000, 64, 20), (256, 256, 128, 3),
     (257, 4099, 64, 32), (300, 33, 200, 32), (513, 30011, 64, 5), (1100, 5000, 100, 8)])
-def test_head_scores(dtype, rows, V, K, top):
+def test_head_scores(form, dtype, rows, V, K, top):
     h, w, tokens, dh, dw, dt = head_case(rows, V, K, rows + V, getattr(torch, dtype))
     head = make_head(dw, getattr(torch, dtype))
     got = head.score(dh, dt, top)
@@ -197,7 +205,7 @@ def test_head_scores(dtype, rows, V, K, top):
 
 @pytest.mark.parametrize("rows", [5, 200, 300])
 @pytest.mark.parametrize("scale,cap", [(0.25, 0.0), (1.0, 3.0), (1.7, 5.0), (-1.0, 0.0), (0.0, 0.0)])
-def test_head_scale_and_cap(rows, scale, cap):
+def test_head_scale_and_cap(form, rows, scale, cap):
     """The factor and the cap round: once a product, and for the cap by the division, tanhf (2 units,
     its documented bound) and the product: 4 roundings of at most the cap's size."""
     h, w, tokens, dh, dw, dt = head_case(rows, 3000, 128, 7, torch.bfloat16)
@@ -212,7 +220,7 @@ def test_head_scale_and_cap(rows, scale, cap):
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("rows", [3, 140, 270])
-def test_head_ordinary_values(dtype, rows):
+def test_head_ordinary_values(form, dtype, rows):
     """Values that do round: a logit may be off by a rounding of 2^-23 a product added up."""
     rng = np.random.default_rng(rows)
     t = getattr(torch, dtype)
@@ -226,7 +234,7 @@ def test_head_ordinary_values(dtype, rows):
 
 
 @pytest.mark.parametrize("rows", [4, 200])
-def test_head_strides_limit_and_ties(rows):
+def test_head_strides_limit_and_ties(form, rows):
     """Rows that lie apart, ids below a limit, and a vocabulary whose every row stands twice."""
     h, w, tokens, dh, dw, dt = head_case(rows, 2000, 64, 11, torch.bfloat16)
     w[1000:] = w[:1000]
@@ -246,7 +254,7 @@ def test_head_strides_limit_and_ties(rows):
 
 
 @pytest.mark.parametrize("rows", [6, 300])
-def test_head_broken_rows(rows):
+def test_head_broken_rows(form, rows):
     """A row with an infinity or a NaN has no distribution; its neighbours keep theirs."""
     h, w, tokens, dh, dw, dt = head_case(rows, 3000, 64, 13, torch.bfloat16)
     head = make_head(dw, torch.bfloat16)
@@ -261,13 +269,32 @@ def test_head_broken_rows(rows):
         assert torch.equal(a[~bad], b[~bad])
 
 
-def test_head_of_no_rows():
+def test_bands_of_stored_rows(monkeypatch):
+    """Rows that go through memory in several bands."""
+    monkeypatch.setattr(embedding, "SCORE_BAND", 1)
+    h, w, tokens, dh, dw, dt = head_case(600, 300, 64, 23, torch.float32)
+    oracle.check(make_head(dw, torch.float32).score(dh, dt, 5), h @ w.T, tokens, 5)
+
+
+def test_more_rows_than_a_launch(form):
+    """More row blocks than a launch takes, the last one ragged."""
+    h, w, tokens, dh, dw, dt = head_case(64 * 256 + 301, 90, 64, 29, torch.bfloat16)
+    got = make_head(dw, torch.bfloat16).score(dh, dt, 3)
+    x = h @ w.T
+    logp = x - x.max(1, keepdims=True)
+    logp -= np.log(np.exp(logp).sum(1, keepdims=True))
+    # of 90 logits within 20 of the greatest: a few units of 2^-24 of each
+    assert np.abs(got.logprobs.cpu().numpy() - logp[np.arange(len(x)), tokens]).max() < 2e-5
+    assert np.array_equal(got.top_ids.cpu().numpy(), np.argsort(-x, axis=1, kind="stable")[:, :3])
+
+
+def test_head_of_no_rows(form):
     _, _, _, dh, dw, dt = head_case(1, 300, 64, 17, torch.bfloat16)
     got = make_head(dw, torch.bfloat16).score(dh[:0], dt[:0], 4)
     assert got.logprobs.shape == (0,) and got.top_ids.shape == (0, 4)
 
 
-def test_head_twice_and_in_graphs():
+def test_head_twice_and_in_graphs(form):
     _, _, _, dh, dw, dt = head_case(300, 9000, 128, 19, torch.bfloat16)
     head = make_head(dw, torch.bfloat16)
     want = head.score(dh, dt, 20)
