@@ -21,6 +21,7 @@ PAGE = 64  # positions per cache page (MB_PAGE in csrc/common.cuh)
 
 _c = ctypes
 _vp, _i, _f, _d, _ll = _c.c_void_p, _c.c_int, _c.c_float, _c.c_double, _c.c_longlong
+_addr = _c.c_ulonglong     # an address that is never None: quicker to hand over than a void pointer
 
 
 def code_of(dtype: torch.dtype) -> int:
@@ -1506,14 +1507,16 @@ def sample(logits: torch.Tensor, temperature: float, state_index: torch.Tensor,
 TOP_SCORES = 32          # alternatives of a row at most (MB_SCORES_TOP in csrc/scores.cuh)
 
 
+_TOKEN_SCORES = [_addr, _ll, _i, _i, _addr, _i, _addr, _addr, _addr, _addr, _i, _addr]
+
+
 def token_scores(logits: torch.Tensor, vocab: int, tokens: torch.Tensor, top: int, out) -> None:
     """Per row of ``logits`` [rows, >= vocab] (float32, a row's values side by side): the log
     probability of ``tokens[row]`` (int32; NaN where that is no id below ``vocab``), the entropy, and
     the ids and log probabilities of the ``top`` greatest logits, the lowest id first among equals,
     into ``out``, a ``sampling.Scores`` of that many rows and alternatives (``token_scores`` there is
     what checks all this)."""
-    _call("scores", "mb_token_scores",
-          [_vp, _ll, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp],
+    _call("scores", "mb_token_scores", _TOKEN_SCORES,
           logits.data_ptr(), logits.stride(0), logits.shape[0], vocab, tokens.data_ptr(), top,
           out.logprobs.data_ptr(), out.entropy.data_ptr(), out.top_ids.data_ptr(),
           out.top_logprobs.data_ptr(), _sms(), _stream())
@@ -1547,12 +1550,18 @@ def head_scores(h: torch.Tensor, w: torch.Tensor, limit: int, scale: float, cap:
 
 
 # ------------------------------------------------------------------------------ a step's arrays
-def _not_a_list(what: str, t: torch.Tensor, n: int) -> KernelError:
-    return KernelError(f"{what}: {t.dtype} {tuple(t.shape)} on {t.device}, not a contiguous int32 list of "
-                       f"{n} beside the others")
-
-
 _int32 = torch.int32
+_STEP_INDEX = [_addr, _addr, _addr, _i, _ll, _addr, _addr, _addr, _addr, _addr]
+_MAP_PAGES = [_addr, _i, _i, _addr, _addr, _addr, _addr, _i, _addr, _i, _i, _addr]
+
+
+def _refuse_lists(what: str, device: int, *lists) -> None:
+    """Raises for the first (tensor, length) that is no contiguous int32 list of that length there."""
+    for t, n in lists:
+        if (t.dtype is not _int32 or t.dim() != 1 or t.numel() != n or t.get_device() != device
+                or not t.is_contiguous()):
+            raise KernelError(f"{what}: {t.dtype} {tuple(t.shape)} on {t.device}, not a contiguous int32 "
+                              f"list of {n} beside the others")
 
 
 def step_index(slots: torch.Tensor, past: torch.Tensor, new: torch.Tensor, seq_start: torch.Tensor,
@@ -1563,15 +1572,24 @@ def step_index(slots: torch.Tensor, past: torch.Tensor, new: torch.Tensor, seq_s
     the step (what lies behind it is left) or shorter (what does not fit is not written). All
     int32, on the device; nothing is read on the host."""
     B, T, device = slots.numel(), tok_seq.numel(), slots.get_device()
-    for t, n in ((slots, B), (past, B), (new, B), (seq_start, B + 1), (tok_seq, T), (tok_pos, T),
-                 (tok_slot, T)):
-        if (t.dtype is not _int32 or t.numel() != n or t.dim() != 1 or t.get_device() != device
-                or not t.is_contiguous()):
-            raise _not_a_list("step_index", t, n)
+    # (one expression: a step of a few tokens waits for the host)
+    if not (slots.dtype is past.dtype is new.dtype is seq_start.dtype is tok_seq.dtype is tok_pos.dtype
+            is tok_slot.dtype is _int32
+            and B == past.numel() == new.numel() == seq_start.numel() - 1
+            and T == tok_pos.numel() == tok_slot.numel()
+            and 1 == slots.dim() == past.dim() == new.dim() == seq_start.dim() == tok_seq.dim()
+            == tok_pos.dim() == tok_slot.dim()
+            and device == past.get_device() == new.get_device() == seq_start.get_device()
+            == tok_seq.get_device() == tok_pos.get_device() == tok_slot.get_device()
+            and slots.is_contiguous() and past.is_contiguous() and new.is_contiguous()
+            and seq_start.is_contiguous() and tok_seq.is_contiguous() and tok_pos.is_contiguous()
+            and tok_slot.is_contiguous()):
+        _refuse_lists("step_index", device, (slots, B), (past, B), (new, B), (seq_start, B + 1),
+                      (tok_seq, T), (tok_pos, T), (tok_slot, T))
     if elsewhere(device):
         with on_device_of(slots):
             return step_index(slots, past, new, seq_start, tok_seq, tok_pos, tok_slot)
-    _call("step_index", "mb_step_index", [_vp, _vp, _vp, _i, _ll, _vp, _vp, _vp, _vp, _vp],
+    _call("step_index", "mb_step_index", _STEP_INDEX,
           slots.data_ptr(), past.data_ptr(), new.data_ptr(), B, T, seq_start.data_ptr(),
           tok_seq.data_ptr(), tok_pos.data_ptr(), tok_slot.data_ptr(), _stream())
 
@@ -1584,10 +1602,14 @@ def map_pages(table: torch.Tensor, slots: torch.Tensor, past: torch.Tensor, new:
     after sequence. Distinct slots. Entries outside the table are left, and so are those that ``pages``
     is too short for. All int32, on the device; nothing is read on the host."""
     B, N, device = slots.numel(), pages.numel(), slots.get_device()
-    for t, n in ((slots, B), (past, B), (new, B), (held, B), (pages, N)):
-        if (t.dtype is not _int32 or t.numel() != n or t.dim() != 1 or t.get_device() != device
-                or not t.is_contiguous()):
-            raise _not_a_list("map_pages", t, n)
+    if not (slots.dtype is past.dtype is new.dtype is held.dtype is pages.dtype is _int32
+            and B == past.numel() == new.numel() == held.numel()
+            and 1 == slots.dim() == past.dim() == new.dim() == held.dim() == pages.dim()
+            and device == past.get_device() == new.get_device() == held.get_device()
+            == pages.get_device()
+            and slots.is_contiguous() and past.is_contiguous() and new.is_contiguous()
+            and held.is_contiguous() and pages.is_contiguous()):
+        _refuse_lists("map_pages", device, (slots, B), (past, B), (new, B), (held, B), (pages, N))
     if (table.dtype is not _int32 or table.dim() != 2 or not table.is_contiguous()
             or table.get_device() != device):
         raise KernelError(f"map_pages: the table is {table.dtype} {tuple(table.shape)} on "
@@ -1598,8 +1620,7 @@ def map_pages(table: torch.Tensor, slots: torch.Tensor, past: torch.Tensor, new:
         with on_device_of(slots):
             return map_pages(table, slots, past, new, held, pages, ring_pages)
     n_slots, max_pages = table.shape
-    _call("step_index", "mb_map_pages",
-          [_vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _vp],
+    _call("step_index", "mb_map_pages", _MAP_PAGES,
           table.data_ptr(), n_slots, max_pages, slots.data_ptr(), past.data_ptr(), new.data_ptr(),
           held.data_ptr(), B, pages.data_ptr(), N, ring_pages, _stream())
 
@@ -1611,8 +1632,7 @@ def map_pages_packed(table: torch.Tensor, lists: torch.Tensor, at: int, B: int, 
     assert lists.dtype == table.dtype == torch.int32 and at + 4 * B + N <= lists.numel()
     p = lists.data_ptr() + 4 * at
     n_slots, max_pages = table.shape
-    _call("step_index", "mb_map_pages",
-          [_vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _vp],
+    _call("step_index", "mb_map_pages", _MAP_PAGES,
           table.data_ptr(), n_slots, max_pages, p, p + 4 * B, p + 8 * B, p + 12 * B, B, p + 16 * B, N,
           ring_pages, _stream())
 
