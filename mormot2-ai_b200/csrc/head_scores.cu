@@ -14,6 +14,8 @@
 #include "scores.cuh"
 #include "tc_common.cuh"
 
+#include <initializer_list>
+
 MB_DEFINE_LAST_ERROR
 
 #define HS_THREADS 192
@@ -493,18 +495,23 @@ static int parts_of(const HeadPlan& plan) {
 
 // Whether mb_head_scores takes operands of these sizes and alignments on this device.
 MB_EXPORT int mb_head_scores_supported(const void* A, int lda, const void* W, int K, int sms) {
-  return K > 0 && K % 8 == 0 && lda % 8 == 0 && ((uintptr_t)A & 15) == 0 && ((uintptr_t)W & 15) == 0 &&
+  return K > 0 && K % 8 == 0 && lda >= K && lda % 8 == 0 && ((uintptr_t)A & 15) == 0 && ((uintptr_t)W & 15) == 0 &&
          head_pairs(sms) > 0;
 }
 
-// bytes of scratch that mb_head_scores needs
+// bytes of scratch that mb_head_scores needs: what the larger of its two plans takes (that of whole
+// launches, and that of the last one, which may be cut into more strips)
 MB_EXPORT long long mb_head_scores_scratch(int rows, int limit, int top, int sms) {
-  const int pairs = head_pairs(sms);
+  const int pairs = head_pairs(sms), most = HS_BLOCKS * 256;
   if (pairs <= 0 || rows <= 0 || limit <= 0) return 0;
-  HeadPlan plan;
-  const int most = HS_BLOCKS * 256;
-  plan_bands(plan, ((rows < most ? rows : most) + 255) / 256, pairs, limit);
-  return (long long)parts_of(plan) * (12 + 8 * top) + 4ll * (rows < most ? rows : most) + 16;
+  long long parts = 0;
+  for (const int n : {rows < most ? 0 : most, rows % most}) {
+    if (n == 0) continue;
+    HeadPlan plan;
+    plan_bands(plan, (n + 255) / 256, pairs, limit);
+    if (parts_of(plan) > parts) parts = parts_of(plan);
+  }
+  return parts * (12 + 8 * top) + 4ll * (rows < most ? rows : most) + 16;
 }
 
 // For rows A [rows, K] (bfloat16, `lda` values from row to row) and a head W [V, K]: the scores of

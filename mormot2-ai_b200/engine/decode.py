@@ -68,7 +68,7 @@ class DecodeRun:
             self.top = top
             self.score_box = torch.empty(n, dtype=torch.int32, device=rt.device)
             self.scores = Scores.packed(self.score_box, ctx.B, top)
-            self.score_ring = torch.empty((self.DEPTH, n), dtype=torch.int32).pin_memory()
+            self.score_ring = torch.empty((self.DEPTH, n), dtype=torch.int32, pin_memory=True)
 
     # ------------------------------------------------------------------ stepping
     def launch(self) -> None:

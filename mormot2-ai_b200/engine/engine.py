@@ -339,7 +339,7 @@ class Engine:
             given = torch.from_numpy(scoring.given.astype(np.int32)).to(self.rt.device)
         elif n_want and len(passes) > 1:
             out = torch.empty((n_want, self.vocab_size), dtype=torch.float32, device=self.rt.device)
-        self.last_h2d_bytes = 0
+        self.last_h2d_bytes = 0 if given is None else 4 * given.numel()
         self.last_passes = len(passes)
         touched = None
         if self.has_state:

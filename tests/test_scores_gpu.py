@@ -194,7 +194,7 @@ def head_case(rows, V, K, seed, dtype):
 @pytest.mark.parametrize("rows,V,K,top", [
     (1, 257, 64, 5), (1, 40000, 128, 32), (16, 1000, 96, 1), (17, 3001, 64, 0), (64, 5003, 192, 20),
     (65, 2048, 72, 7), (128, 509, 256, 32), (129, 700, 64, 5), (255, 20000, 64, 20), (256, 256, 128, 3),
-    (257, 4099, 64, 32), (300, 33, 200, 32), (513, 30011, 64, 5), (1100, 5000, 100, 8)])
+    (257, 4099, 64, 32), (300, 33, 200, 32), (70, 7, 64, 7), (40, 1, 64, 1), (513, 30011, 64, 5), (1100, 5000, 100, 8)])
 def test_head_scores(form, dtype, rows, V, K, top):
     h, w, tokens, dh, dw, dt = head_case(rows, V, K, rows + V, getattr(torch, dtype))
     head = make_head(dw, getattr(torch, dtype))
@@ -276,9 +276,11 @@ def test_bands_of_stored_rows(monkeypatch):
     oracle.check(make_head(dw, torch.float32).score(dh, dt, 5), h @ w.T, tokens, 5)
 
 
-def test_more_rows_than_a_launch(form):
-    """More row blocks than a launch takes, the last one ragged."""
-    h, w, tokens, dh, dw, dt = head_case(64 * 256 + 301, 90, 64, 29, torch.bfloat16)
+@pytest.mark.parametrize("more", [301, 37 * 256 - 3])
+def test_more_rows_than_a_launch(form, more):
+    """More row blocks than a launch takes, the last launch ragged (37 blocks are cut into more parts than
+    64 are)."""
+    h, w, tokens, dh, dw, dt = head_case(64 * 256 + more, 90, 64, 29, torch.bfloat16)
     got = make_head(dw, torch.bfloat16).score(dh, dt, 3)
     x = h @ w.T
     logp = x - x.max(1, keepdims=True)
