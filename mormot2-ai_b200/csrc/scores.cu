@@ -46,17 +46,24 @@ __device__ __forceinline__ float warp_nth(float v, int top) {
   return least;
 }
 
-#define SC_FEW 8       // alternatives up to which the warps' bars are near enough
+// The `nth` greatest of the warp's values, each lane one, for a small `nth`
+__device__ __forceinline__ float warp_few(float v, int nth) {
+  const int lane = threadIdx.x & 31;
+  float m = warp_max(v);
+  for (int i = 1; i < nth; ++i) {
+    if (lane == __ffs(__ballot_sync(0xffffffffu, v == m)) - 1) v = -INFINITY;
+    m = warp_max(v);
+  }
+  return m;
+}
 
 struct ScShared {
   float best[SC_WARPS], bar[SC_WARPS];
   alignas(16) uint32_t place[SC_ROOM];      // of the keys held, in order, and of those that passed the bar
   uint32_t id[SC_ROOM];                     // and their ids
-  alignas(16) uint32_t heads[SC_THREADS];   // the threads' greatest values that passed the warps' bars
   TopKey sorted[MB_SCORES_TOP], pick[SC_WARPS];
-  int taken[MB_SCORES_TOP], passed[3], n_heads, equal[2];
-  uint32_t least;
-  Mass part[SC_WARPS];
+  int taken[MB_SCORES_TOP], passed[3], equal[2];
+  float most[SC_WARPS], s[SC_WARPS], t[SC_WARPS];
   // of the cluster's first CTA: every CTA's part
   Mass mass[SC_CLUSTER];
   alignas(16) uint32_t all_place[SC_CLUSTER * MB_SCORES_TOP];
@@ -162,9 +169,10 @@ __device__ __noinline__ void sc_pick(const float* __restrict__ x, int base, int 
 // What a CTA finds in its part of a row, x[0 .. n) with ids from id0 on: the mass (every thread has it),
 // and in sh.sorted the greatest `top` keys in order, 0 where there are no more finite values.
 //
-// The first round sets a bar that few values pass and the `top` greatest do: each warp knows the `top`-th
-// of its 32 threads' greatest values, and the highest of these bars holds for the block. From then on
-// the bar is the `top`-th greatest value so far, which hardly any value passes, and a round costs what the
+// The first round sets a bar that few values pass and the `top` greatest do: with every warp's ceil(top / 8)
+// greatest threads there are `top`, so the least of these threads' greatest values is one (of 10,240 values
+// some 45 pass it for 20 alternatives, where the `top`-th thread of the best warp lets 200 pass). From then
+// on the bar is the `top`-th greatest value so far, which hardly any value passes, and a round costs what the
 // sums cost, and one barrier. Each thread's sums are over the greatest value that it has seen itself.
 template <int EACH, bool WIDE, bool TOP>
 __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int id0, int top, int& turn, ScShared& sh) {
@@ -175,7 +183,7 @@ __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int 
   int held = 0, third = 0;             // keys in sh.sorted; the round's counter of three
   if (TOP) {
     if (threadIdx.x < MB_SCORES_TOP) sh.taken[threadIdx.x] = 0;
-    if (threadIdx.x == 0) sh.passed[0] = sh.n_heads = sh.equal[0] = 0, sh.least = ~0u;
+    if (threadIdx.x == 0) sh.passed[0] = sh.equal[0] = 0;
   }
   for (int base = 0; base < n; base += ROUND) {
     float v[EACH];
@@ -184,21 +192,22 @@ __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int 
 #pragma unroll
     for (int i = 1; i < EACH; ++i) best = fmaxf(best, v[i]);
     if (TOP && base == 0) {
-      const float nth = top == 1 ? warp_max(best) : warp_nth(best, top);
-      if (lane == 0) sh.bar[warp] = nth;
+      // Every warp's so many greatest threads together are `top` threads or more (for one, the best will do).
+      const float few = warp_few(best, (top + SC_WARPS - 1) / SC_WARPS);
+      if (lane == 0) sh.best[warp] = few > -INFINITY ? few : -INFINITY;       // (a NaN is none)
       __syncthreads();
+      float least = sh.best[0];
 #pragma unroll
-      for (int w = 0; w < SC_WARPS; ++w) bar = fmaxf(bar, sh.bar[w]);
-      if (top > SC_FEW) {
-        // The `top`-th of all threads' greatest values is a bar as well, which fewer pass; only those that
-        // pass the warps' bars (at least `top` do, if so many are finite) can be above it.
-        const uint32_t p = key_place(best);
-        if (best >= bar) sh.heads[atomicAdd(&sh.n_heads, 1)] = p;
+      for (int w = 1; w < SC_WARPS; ++w) least = top == 1 ? fmaxf(least, sh.best[w]) : fminf(least, sh.best[w]);
+      if (least > -INFINITY) {
+        bar = fmaxf(bar, least);
+      } else {
+        // a warp without so many finite values: the `top`-th of the best warp's threads
+        const float nth = warp_nth(best, top);
+        if (lane == 0) sh.bar[warp] = nth;
         __syncthreads();
-        const int heads = sh.n_heads;
-        if (best >= bar && sc_above(sh.heads, heads, p) < top) atomicMin(&sh.least, p);
-        __syncthreads();
-        if (heads >= top) bar = key_value((TopKey)sh.least << 32);
+#pragma unroll
+        for (int w = 0; w < SC_WARPS; ++w) bar = fmaxf(bar, sh.bar[w]);
       }
     }
     if (TOP && best >= bar) {
@@ -241,10 +250,21 @@ __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int 
     if (held == top) bar = key_value(((sh.sorted[top - 1] >> 32) + 1) << 32);
   }
   if (TOP && threadIdx.x < top && threadIdx.x >= held) sh.sorted[threadIdx.x] = 0;
-  mine = mass_warp(mine);
-  if (lane == 0) sh.part[warp] = mine;
+  const float most_warp = warp_max(mine.m);
+  if (lane == 0) sh.most[warp] = most_warp;
   __syncthreads();
-  return mass_warp(lane < SC_WARPS ? sh.part[lane] : mass_none());
+  float most = sh.most[0];
+#pragma unroll
+  for (int w = 1; w < SC_WARPS; ++w) most = fmaxf(most, sh.most[w]);
+  mine = mass_over(mine, most);
+  mine.s = warp_sum(mine.s);
+  mine.t = warp_sum(mine.t);
+  if (lane == 0) sh.s[warp] = mine.s, sh.t[warp] = mine.t;
+  __syncthreads();
+  mine = {most, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < SC_WARPS; ++w) mine.s += sh.s[w], mine.t += sh.t[w];
+  return mine;
 }
 
 template <int EACH, int CTAS, bool TOP>
