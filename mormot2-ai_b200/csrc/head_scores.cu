@@ -6,11 +6,21 @@
 // A CTA pair (rank 0 issues tcgen05.mma.cta_group::2 for both) keeps 256 rows and walks a strip of
 // the vocabulary in tiles of up to 256 ids; 128 threads a CTA own a row each and fold a tile from
 // tensor memory into their row's mass and keys while the next tile is multiplied. At the strip's end
-// they leave both in memory; a block a row joins the strips (score_join_kernel in scores.cuh).
+// they leave both in memory; a warp a row joins the strips (head_join_kernel).
 //
 // The pairs that share a strip walk it side by side, so that its weights come from memory once and from
 // L2 for all row blocks but the first: a band of b row blocks takes floor(pairs / b) strips. Rows are
 // cut into bands such that few pairs idle (plan_bands).
+//
+// Bound: the tensor cores, from K of some 1,500 on (rows padded to 256; 151,936 ids, 5 alternatives: 1,024 rows of
+// 4,096 values 804 us with the tensor pipe 98 % active, weights read once, 1.30 GB; 2,048 rows again and
+// again 1.35 PFLOP/s under the power cap, on rows of few bits 1.53). Below that the four warps that read
+// tensor memory: some 550 cycles for 32 ids of a row (the exponentials alone take 256), and with 5 or 20
+// alternatives 280 or 700 more, most of them in the first tiles (1,024 values a row, 2,048 rows: 406, 475 and
+// 650 us). Up to 128 rows the head's bytes (1,024 values: 60 us, 5.2 TB/s).
+// Taken back: two such warps a quarter of the lanes, a tile each in turn (their lists see half the ids each,
+// and together nearly twice the new values: 501 us, 656 with 20); ids in a log beside the values in
+// registers (810 with 20: every value's way to the log is a branch).
 #include "scores.cuh"
 #include "tc_common.cuh"
 
@@ -128,8 +138,9 @@ __device__ __forceinline__ void load32(uint32_t taddr, float* x) {
 }
 // cap tanh(x / cap). For |u| up to 1 the continued fraction u / (1 + u^2 / (3 + u^2 / (5 + ...)))
 // (Lambert) cut behind the 9 gives u (945 + 105 u^2 + u^4) / (945 + 420 u^2 + 15 u^4), off by less than
-// 4 units of 2^-24; beyond it the exponential's form is exact enough. tanhf and a division took 3 us a tile of
-// 256 ids and, for the zeros of rows that are not there, 9.
+// 4 units of 2^-24; beyond it the exponential's form is exact enough. With tanhf and a division 333 rows of
+// 2,048 values took 957 us where this takes 210 (a division of 0 has a way of its own, which the rows that
+// are not there took).
 __device__ __forceinline__ float capped_small(float x, float cap, float by) {
   const float u = x * by, z = u * u;
   return cap * __fdividef(u * fmaf(z, z + 105.f, 945.f), fmaf(z, fmaf(z, 15.f, 420.f), 945.f));
@@ -462,7 +473,10 @@ static int strip_width(int blocks, int pairs, int limit) {
 }
 
 // Cuts `blocks` row blocks into bands of at most `pairs` blocks such that the strips' widths add up
-// to the least: the time of a band is that of its widest strip, and a strip's start and end.
+// to the least: the time of a band is that of its widest strip, and a strip's start and end (its first tile
+// has nothing to overlap, its last one's values neither), which count as 512 ids. With 64 the 2,048 rows
+// above took four bands of two blocks, which fill the pairs exactly and read the weights four times: 2,090 us
+// where one band of eight takes 1,885, with 1,024 values 623 and 475.
 static void plan_bands(HeadPlan& plan, int blocks, int pairs, int limit) {
   int best[HS_BLOCKS + 1], take[HS_BLOCKS + 1];
   best[0] = 0;

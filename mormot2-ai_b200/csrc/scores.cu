@@ -3,6 +3,13 @@
 // to eight CTAs shares a row, a thread holds 24 or 40 values of it at a time. They are added up over the
 // thread's maximum; the alternatives are picked out by a bar that at least `top` of them pass. The cluster's
 // first CTA then joins the parts through distributed shared memory, so that one launch does it all.
+//
+// Bound: many rows by the logits' bytes (2,048 rows of 151,936: 175 us without alternatives, 7.1 TB/s, 198 with
+// 5, 226 with 20); few rows by the chain of barriers from the first value to the last sum (one row: 4.1 us
+// without, 8.3 with 5). Taken back: CTAs that stay for several rows and ask for the next row ahead (the
+// values asked for take the registers of a CTA: 303 us where CTAs that go take 223), the rest of a row
+// brought into L2 while the first values are looked at (237), a place in the list for a whole warp at a time
+// (204), keys put in order only at a part's end (273 where every round's take 265).
 #include "scores.cuh"
 
 MB_DEFINE_LAST_ERROR
@@ -332,11 +339,12 @@ MB_EXPORT int mb_token_scores(const float* logits, long long stride, int rows, i
   if (rows <= 0) return 0;
   if (V <= 0 || top < 0 || top > MB_SCORES_TOP || top > V)
     MB_FAIL("mb_token_scores: %d alternatives of a vocabulary of %d", top, V);
-  // Where a row in eight parts for each of a few rows fits the device at once, 40 values a thread make the
-  // fewest rounds; else 24 leave room for a fifth CTA on a multiprocessor, whose loads cover the others'
-  // barriers. 151,936 values, 5 alternatives, us with 40 | 24: 1 row 8.8 | 11.0, 64 rows 16 | 20, 300 rows
-  // 59 | 43, 2,048 rows 223 | 201; 2,048 rows of 4,000 values 31 | 26.
-  const bool few = (long long)rows * SC_CLUSTER <= 4 * sms;
+  // 24 values a thread leave room for five CTAs on a multiprocessor, whose loads cover each other's barriers;
+  // where a few rows in eight parts each fit the device at once all the same, and a part would take three
+  // rounds of 24, it takes fewer of 40. 5 alternatives, us with 40 | 24: of 151,936 values 1 row 8.1 | 10.2,
+  // 64 rows 15.6 | 17.3, 300 rows 54 | 42, 2,048 rows 220 | 197; 37 rows of 50,257 8.9 | 8.7, 64 of 32,768
+  // 9.1 | 7.9.
+  const bool few = (long long)rows * SC_CLUSTER <= 4 * sms && V > 65536;
   // As many parts a row as make the rounds of CTAs the shortest, a part's start and end counting as 4,096
   // values, and none of less than 2,048.
   const int slots = (few ? 4 : 5) * sms;
