@@ -1,10 +1,12 @@
 """Scores through the engine, the client and the command line: given texts, and the tokens of answers."""
+import importlib
+
 import numpy as np
 import pytest
-import torch
 
 from mormot2_ai_b200 import CacheError, Engine, Entry, InferError, LlmClient, Sampling
 from mormot2_ai_b200.cli import main
+from mormot2_ai_b200.parts import embedding
 from mormot2_ai_b200.sampling import DeviceSampler
 from tests import score_oracle as oracle
 
@@ -69,6 +71,43 @@ def test_score_token_by_token(tiny, dtype):
     assert got.logprobs.shape == (0,) and got.top_ids.shape == (0, 2)
     assert eng.length(slots[0]) == 9 and eng.length(slots[1]) == 10
     eng.rt.check()
+
+
+FAMILIES = ["busavik", "fimudra", "sezopel", "laralix", "lotirax", "tenusun"]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("family", FAMILIES)
+def test_every_family_scores(family, dtype, tmp_path, monkeypatch):
+    """Heads with a factor or capped logits, states, several passes: the fused form and the stored one
+    against the logits of a step of the same engine."""
+    models = importlib.import_module(f"tests.{family}_models")
+    for name in models.SMALL:
+        small = models.SmallModel(name, str(tmp_path / name))
+        eng = Engine.from_folder(small.folder, dtype=dtype, max_tokens=1024, max_slots=3, prefill_chunk=40)
+        head, norms = eng.model.head, []
+        forward = head.forward
+
+        def watched(h):
+            norms.append(float(h.double().norm(dim=1).max()))
+            return forward(h)
+        texts = [small.tokens(n, seed=n) for n in (70, 3, 41)]
+        slots = [eng.open() for _ in texts]
+        head.forward = watched
+        x = eng.step([Entry(s, t, list(range(len(t) - 1))) for s, t in zip(slots, texts)])
+        head.forward = forward
+        x = x.double().cpu().numpy()
+        w = head.linear.weight.double()
+        # the products' order, the factor, the cap (a division, tanh and a product, each side its own)
+        off = abs(head.scale) * w.shape[1] * 2.0 ** -23 * max(norms) * float(w.norm(dim=1).max())
+        off += 2.0 ** -23 * np.abs(x).max() + 2.0 ** -23 * 8 * head.softcap
+        for fused in (False, True):
+            monkeypatch.setattr(embedding, "scores_through_memory", lambda *sizes: not fused)
+            for s in slots:
+                eng.truncate(s, 0)
+            got = eng.score([Entry(s, t) for s, t in zip(slots, texts)], top=6)
+            eng.rt.check()
+            oracle.check(got, x, [t for one in texts for t in one[1:]], 6, off)
 
 
 def test_score_refusals(tiny_a_model):
