@@ -66,9 +66,9 @@ class DecodeRun:
                 raise InferError("a run that keeps its picks on the device does not score them")
             n = ctx.B * (2 + 2 * top)
             self.top = top
-            self.score_box = torch.empty(n, dtype=torch.int32, device=rt.device)
-            self.scores = Scores.packed(self.score_box, ctx.B, top)
-            self.score_ring = torch.empty((self.DEPTH, n), dtype=torch.int32, pin_memory=True)
+            self.score_box = torch.empty(n, dtype=torch.float32, device=rt.device)
+            self.scores = Scores.in_buffer(self.score_box, ctx.B, top)
+            self.score_ring = torch.empty((self.DEPTH, n), dtype=torch.float32, pin_memory=True)
 
     # ------------------------------------------------------------------ stepping
     def launch(self) -> None:
@@ -103,7 +103,7 @@ class DecodeRun:
         if self.scores is not None:                 # copied ahead of the picks
             ring = self.score_ring[self.n_read % self.DEPTH]
             self.last_scores = self._in_slot_order(
-                Scores.packed(ring, self.ctx.B, self.top).on_host())
+                Scores.in_buffer(ring, self.ctx.B, self.top).on_host())
             self.d2h_bytes += 4 * ring.numel()
         got = self._in_slot_order(got)
         self.n_read += 1

@@ -70,21 +70,21 @@ def test_map_pages_refusals():
         K.map_pages(*good)
 
 
-def test_packed_scores():
-    buffer = torch.arange(3 * (2 + 2 * 4), dtype=torch.int32)
-    s = Scores.packed(buffer, 3, 4)
+def test_scores_in_a_buffer():
+    buffer = torch.arange(3 * (2 + 2 * 4), dtype=torch.int32).view(torch.float32)
+    s = Scores.in_buffer(buffer, 3, 4)
     s.logprobs.copy_(torch.tensor([-1.0, -2.0, -3.0]))
     s.entropy.copy_(torch.tensor([0.5, 1.5, 2.5]))
     s.top_logprobs.copy_(-torch.arange(12.0).view(3, 4))
     assert s.top_ids.tolist() == [[6, 7, 8, 9], [10, 11, 12, 13], [14, 15, 16, 17]]
     rows = s.on_host()
     assert rows[1] == TokenScore(-2.0, 1.5, [(10, -4.0), (11, -5.0), (12, -6.0), (13, -7.0)])
-    copy = Scores.packed(torch.zeros_like(buffer), 3, 4)
+    copy = Scores.in_buffer(torch.zeros_like(buffer), 3, 4)
     copy.put(torch.tensor([2, 0, 1]), s)
     assert copy.logprobs.tolist() == [-2.0, -3.0, -1.0] and copy.top_ids[2].tolist() == [6, 7, 8, 9]
     copy.rows(1, 3).take(s.rows(0, 2))
     assert copy.on_host()[1:] == rows[:2]
-    assert Scores.packed(torch.zeros(6, dtype=torch.int32), 3, 0).on_host()[2] == TokenScore(0.0, 0.0, [])
+    assert Scores.in_buffer(torch.zeros(6), 3, 0).on_host()[2] == TokenScore(0.0, 0.0, [])
 
 
 def test_text_score():

@@ -113,7 +113,7 @@ def test_vocab_limit_and_out():
     oracle.check(out, x, tokens, 6)
     with pytest.raises(InferError):
         token_scores(on_device(x), torch.from_numpy(tokens).to(DEV), 5, None, out)
-    packed = Scores.packed(torch.empty(4 * 14, dtype=torch.int32, device=DEV), 4, 6)
+    packed = Scores.in_buffer(torch.empty(4 * 14 + 3, device=DEV)[3:], 4, 6)
     token_scores(on_device(x), torch.from_numpy(tokens).to(DEV), 6, None, packed)
     for a, b in zip(packed.tensors(), out.tensors()):
         assert torch.equal(a, b)
