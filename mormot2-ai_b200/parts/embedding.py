@@ -91,11 +91,14 @@ class LmHead(Part):
         if K.elsewhere(h.get_device()):
             with K.on_device_of(h):
                 return self.score(h, tokens, top, vocab_limit)
-        rows = h.shape[0]
-        out = Scores.empty(rows, top, h.device)
+        rows, weight, rt = h.shape[0], self.linear.weight, self.linear.rt
+        floats = h if h.dtype == torch.float32 else rt.workspace
+        if floats is None:
+            out = Scores.empty(rows, top, h.device)
+        else:
+            out = Scores.beside(floats, tokens, rows, top)
         if rows == 0:
             return out
-        weight, rt = self.linear.weight, self.linear.rt
         tokens = tokens.contiguous()
         if (self.linear.fast is not None and not scores_through_memory(rows, self.hidden, top)
                 and K.head_scores_supported(h, weight)):
