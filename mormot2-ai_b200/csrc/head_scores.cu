@@ -4,9 +4,10 @@
 // logits is a mass (the maximum, S and T of scores.cuh) and `top` keys.
 //
 // A CTA pair (rank 0 issues tcgen05.mma.cta_group::2 for both) keeps 256 rows and walks a strip of
-// the vocabulary in tiles of up to 256 ids; 128 threads a CTA own a row each and fold a tile from
-// tensor memory into their row's mass and keys while the next tile is multiplied. At the strip's end
-// they leave both in memory; a warp a row joins the strips (head_join_kernel).
+// the vocabulary in tiles of up to 256 ids; up to 128 rows each CTA walks by itself, in tiles of up to 128.
+// 128 threads a CTA own a row each and fold a tile from tensor memory into their row's mass and keys while
+// the next tile is multiplied. At the strip's end they leave both in memory; a warp a row joins the strips
+// (head_join_kernel).
 //
 // The pairs that share a strip walk it side by side, so that its weights come from memory once and from
 // L2 for all row blocks but the first: a band of b row blocks takes floor(pairs / b) strips. Rows are
@@ -17,10 +18,12 @@
 // again 1.35 PFLOP/s under the power cap, on rows of few bits 1.53). Below that the four warps that read
 // tensor memory: some 550 cycles for 32 ids of a row (the exponentials alone take 256), and with 5 or 20
 // alternatives 280 or 700 more, most of them in the first tiles (1,024 values a row, 2,048 rows: 406, 475 and
-// 650 us). Up to 128 rows the head's bytes (1,024 values: 60 us, 5.2 TB/s).
+// 650 us). Up to 128 rows the head's bytes (1,024 values: 57 to 61 us, 5.1 to 5.4 TB/s; 4,096: 222, 5.6).
 // Taken back: two such warps a quarter of the lanes, a tile each in turn (their lists see half the ids each,
 // and together nearly twice the new values: 501 us, 656 with 20); ids in a log beside the values in
-// registers (810 with 20: every value's way to the log is a branch).
+// registers (810 with 20: every value's way to the log is a branch); a CTA by itself with tiles of 256 ids
+// (128 rows of 2,048 values 124 us against 115, of 4,096 242 against 223; four stages instead of six); pairs that
+// copy no rows beyond the last one (129 rows of 1,024 values 66 us against 64).
 #include "scores.cuh"
 #include "tc_common.cuh"
 
@@ -30,41 +33,44 @@ MB_DEFINE_LAST_ERROR
 
 #define HS_THREADS 192
 #define HS_BK 64
+#define HS_HALF (128 * HS_BK * 2)            // 128 rows of an operand in a stage
 #define HS_STAGES 6
-#define HS_HALF (128 * HS_BK * 2)            // one CTA's rows of an operand in a stage
-#define HS_PAIRS 96                          // CTA pairs at most
-#define HS_BLOCKS 64                         // row blocks of 256 of a launch at most
+#define HS_STRIPS 160                        // strips of a row at most
+#define HS_BLOCKS 64                         // row blocks of a launch at most
 #define HS_STAGED (4 * 32 * 128)             // 32 values of 32 rows for each epilogue warp
 #define HS_SMEM (1024 + HS_STAGES * 2 * HS_HALF + 256 + HS_STAGED)
 
+// A CTA pair multiplies 256 rows with 256 ids, each CTA bringing half of both; a CTA by itself 128 with 128.
+__host__ __device__ constexpr int block_rows_of(bool pair) { return pair ? 256 : 128; }
+
 // A band: `blocks` row blocks from `first` on, each in `strips` strips of `width` ids, tiles of `tile`
 struct HeadPlan {
-  int bands;
+  int bands, block_rows;
   int first[HS_BLOCKS], blocks[HS_BLOCKS], strips[HS_BLOCKS], width[HS_BLOCKS], tile[HS_BLOCKS];
-  int part0[HS_BLOCKS];      // where a band's parts begin: [block][256 rows][strips]
+  int part0[HS_BLOCKS];      // where a band's parts begin: [block][row][strips]
 };
 
-// The tiles of a pair, the same for all of its warps
+// The tiles of a pair (or of a CTA by itself), the same for all of its warps
 struct HeadWalk {
   const HeadPlan& plan;
-  int pair, limit, band, block, strip, n, end;
-  __device__ HeadWalk(const HeadPlan& p, int pair_, int limit_) : plan(p), pair(pair_), limit(limit_), band(-1) {
+  int unit, limit, band, block, strip, n, end;
+  __device__ HeadWalk(const HeadPlan& p, int unit_, int limit_) : plan(p), unit(unit_), limit(limit_), band(-1) {
     n = end = 0;
   }
-  // the next strip of the pair; false when there is none
+  // its next strip; false when there is none
   __device__ __forceinline__ bool next_strip() {
     while (++band < plan.bands) {
       const int b = plan.blocks[band];
-      if (pair >= b * plan.strips[band]) continue;
-      block = pair % b;
-      strip = pair / b;
+      if (unit >= b * plan.strips[band]) continue;
+      block = unit % b;
+      strip = unit / b;
       n = strip * plan.width[band];
       end = min(limit, n + plan.width[band]);
       return true;
     }
     return false;
   }
-  __device__ __forceinline__ int row0() const { return (plan.first[band] + block) * 256; }
+  __device__ __forceinline__ int row0() const { return (plan.first[band] + block) * plan.block_rows; }
   __device__ __forceinline__ int cols() const { return min(plan.tile[band], end - n); }
   __device__ __forceinline__ void step() { n += plan.tile[band]; }
 };
@@ -95,6 +101,7 @@ template <int N> struct TopList {
     clear(top);
     if (least > -INFINITY) bar = least - 1e-6f * fabsf(least) - 1e-30f;
   }
+  __device__ __forceinline__ void hush() { bar = INFINITY; }      // a row that is not there
   __device__ __forceinline__ void offer(float x, int i) {
     bool past[N];
 #pragma unroll
@@ -119,6 +126,7 @@ template <> struct TopList<0> {
   __device__ __forceinline__ void clear(int) {}
   __device__ __forceinline__ void probe(float) {}
   __device__ __forceinline__ void start(int) {}
+  __device__ __forceinline__ void hush() {}
   __device__ __forceinline__ void offer(float, int) {}
   __device__ __forceinline__ void write(TopKey*, int) const {}
 };
@@ -173,25 +181,34 @@ __device__ __forceinline__ float max32(const float* x) {
   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
-template <int N>
+// Rows that are copied for a tile of `rows`: by pairs all, those beyond the last one as zeros; by a CTA by itself
+// no more than are there, where the copies' zeros take longer than the weights (1,024 values a row: 4 rows
+// 82 us in a box of 128 rows, 61 in one of 8). Behind them the tile holds whatever was there; nobody reads
+// its products. Pairs multiply for longer than they copy, and zeros are what keeps the tensor cores coolest.
+template <bool PAIR> __host__ __device__ __forceinline__ int box_rows(int rows) {
+  return PAIR ? 128 : (rows + 7) & ~7;
+}
+
+template <int N, bool PAIR>
 __global__ void __launch_bounds__(HS_THREADS, 1)
 head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                   const __grid_constant__ HeadPlan plan, int rows, int limit, int K, float scale,
-                   float cap, const int* __restrict__ tokens, int top, float* __restrict__ given,
-                   Mass* __restrict__ mass, TopKey* __restrict__ keys, int* __restrict__ error) {
+                   const __grid_constant__ HeadPlan plan, int rows, int limit, int K, float scale, float cap,
+                   const int* __restrict__ tokens, int top, float* __restrict__ given, Mass* __restrict__ mass,
+                   TopKey* __restrict__ keys, int* __restrict__ error) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   const uint32_t sA = base, sB = base + HS_STAGES * HS_HALF;
-  const uint32_t bars = sB + HS_STAGES * HS_HALF;
+  const uint32_t bars = base + HS_STAGES * 2 * HS_HALF;
   const uint32_t full0 = bars, empty0 = bars + 8 * HS_STAGES;
   const uint32_t acc_full0 = bars + 16 * HS_STAGES, acc_empty0 = acc_full0 + 16;
   const uint32_t slot = acc_empty0 + 16;
   const uint32_t staged = bars + 256;
   volatile uint32_t* slot_ptr = (volatile uint32_t*)(smem_raw + (slot - raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
+  const uint32_t rank = PAIR ? cluster_rank() : 0;
   const int nkb = (K + HS_BK - 1) / HS_BK;
+  const int row_bytes = box_rows<PAIR>(rows) * HS_BK * 2;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < HS_STAGES; ++s) {
@@ -200,20 +217,22 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full0 + 8 * b, 1);
-      mbar_init(acc_empty0 + 8 * b, 8);      // the epilogue warps of both CTAs
+      mbar_init(acc_empty0 + 8 * b, PAIR ? 8 : 4);      // the epilogue warps (of both CTAs)
     }
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
   }
-  if (warp == 1) tmem_alloc_pair(slot, 512);
+  if (warp == 1) {
+    if (PAIR) tmem_alloc_pair(slot, 512); else tmem_alloc(slot, 512);
+  }
   tc_fence_before_sync();
-  cluster_sync_all();
+  if (PAIR) cluster_sync_all(); else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *slot_ptr;
   mb_grid_wait();
   mb_grid_launch_next();
-  HeadWalk walk(plan, blockIdx.x >> 1, limit);
+  HeadWalk walk(plan, PAIR ? blockIdx.x >> 1 : blockIdx.x, limit);
   if (warp == 0) {
     if (elect_one()) {
       int s = 0;
@@ -221,14 +240,20 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       while (walk.next_strip()) {
         const int m0 = walk.row0() + (int)rank * 128;
         for (; walk.n < walk.end; walk.step()) {
-          // each CTA holds half of the tile's ids (whole boxes of 128 are copied)
+          // each CTA of a pair holds half of the tile's ids (whole boxes of 128 are copied)
           const int n0 = walk.n + (int)rank * (((walk.cols() + 15) & ~15) >> 1);
           for (int i = 0; i < nkb; ++i) {
             mbar_wait(empty0 + 8 * s, ph ^ 1, error, 61);
-            if (rank == 0) mbar_expect_tx(full0 + 8 * s, 4 * HS_HALF);
-            const uint32_t full_lead = cluster_addr_of(full0 + 8 * s, 0);
-            tma_load_2d_pair(sA + s * HS_HALF, &tmA, i * HS_BK, m0, full_lead);
-            tma_load_2d_pair(sB + s * HS_HALF, &tmB, i * HS_BK, n0, full_lead);
+            if (PAIR) {
+              if (rank == 0) mbar_expect_tx(full0 + 8 * s, 4 * HS_HALF);
+              const uint32_t full_lead = cluster_addr_of(full0 + 8 * s, 0);
+              tma_load_2d_pair(sA + s * HS_HALF, &tmA, i * HS_BK, m0, full_lead);
+              tma_load_2d_pair(sB + s * HS_HALF, &tmB, i * HS_BK, n0, full_lead);
+            } else {
+              mbar_expect_tx(full0 + 8 * s, HS_HALF + row_bytes);
+              tma_load_2d(sA + s * HS_HALF, &tmA, i * HS_BK, m0, full0 + 8 * s);
+              tma_load_2d(sB + s * HS_HALF, &tmB, i * HS_BK, n0, full0 + 8 * s);
+            }
             if (++s == HS_STAGES) { s = 0; ph ^= 1; }
           }
         }
@@ -240,7 +265,7 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       uint32_t ph = 0;
       while (walk.next_strip()) {
         for (; walk.n < walk.end; walk.step(), ++it) {
-          const uint32_t idesc = umma_idesc_bf16(256, (walk.cols() + 15) & ~15);
+          const uint32_t idesc = umma_idesc_bf16(block_rows_of(PAIR), (walk.cols() + 15) & ~15);
           const int b = it & 1;
           mbar_wait(acc_empty0 + 8 * b, ((it >> 1) & 1) ^ 1, error, 62);
           tc_fence_after_sync();
@@ -250,12 +275,14 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             const uint64_t da = umma_desc_k128(sA + s * HS_HALF);
             const uint64_t db = umma_desc_k128(sB + s * HS_HALF);
 #pragma unroll
-            for (int k = 0; k < HS_BK / 16; ++k)
-              umma_bf16_pair(tmem + b * 256, da + 2 * k, db + 2 * k, idesc, (i | k) != 0);
-            umma_commit_pair(empty0 + 8 * s, 3);
+            for (int k = 0; k < HS_BK / 16; ++k) {
+              if (PAIR) umma_bf16_pair(tmem + b * 256, da + 2 * k, db + 2 * k, idesc, (i | k) != 0);
+              else umma_bf16(tmem + b * 256, da + 2 * k, db + 2 * k, idesc, (i | k) != 0);
+            }
+            if (PAIR) umma_commit_pair(empty0 + 8 * s, 3); else umma_commit(empty0 + 8 * s);
             if (++s == HS_STAGES) { s = 0; ph ^= 1; }
           }
-          umma_commit_pair(acc_full0 + 8 * b, 3);
+          if (PAIR) umma_commit_pair(acc_full0 + 8 * b, 3); else umma_commit(acc_full0 + 8 * b);
         }
       }
     }
@@ -272,6 +299,7 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       TopList<N> list;
       list.clear(top);
       bool fresh = true;
+      if (row >= rows) list.hush();
       const bool idle = walk.row0() + (int)rank * 128 + q * 32 >= rows;    // none of the warp's rows is there
       for (; walk.n < walk.end; walk.step(), ++it) {
         const int b = it & 1, cols = walk.cols();
@@ -297,6 +325,7 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             }
           }
           list.start(top);
+          if (row >= rows) list.hush();
         }
 #pragma unroll 1
         for (int c = 0; c < (idle ? 0 : cols); c += 32) {
@@ -354,20 +383,23 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       }
       if (row < rows) {
         const int strips = plan.strips[walk.band];
-        const size_t part = plan.part0[walk.band] + ((size_t)walk.block * 256 + in_block) * strips + walk.strip;
+        const size_t part =
+            plan.part0[walk.band] + ((size_t)walk.block * block_rows_of(PAIR) + in_block) * strips + walk.strip;
         mass[part] = {m, s, t};
         list.write(keys + part * top, top);
       }
     }
   }
-  // neither CTA leaves while the other may still read its shared memory or signal its barriers
+  // neither CTA of a pair leaves while the other may still read its shared memory or signal its barriers
   tc_fence_before_sync();
-  cluster_sync_all();
-  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+  if (PAIR) cluster_sync_all(); else __syncthreads();
+  if (warp == 1) {
+    if (PAIR) tmem_dealloc_pair(tmem, 512); else tmem_dealloc(tmem, 512);
+  }
 }
 
 // A warp a row joins its strips: their masses, and `top` times the greatest of the heads of their keys,
-// which are in order. A lane has the strips lane, lane + 32 and lane + 64.
+// which are in order. A lane has the strips lane, lane + 32 and so on.
 __global__ void __launch_bounds__(32)
 head_join_kernel(const __grid_constant__ HeadPlan plan, const Mass* __restrict__ mass,
                  const TopKey* __restrict__ keys, int top, const float* __restrict__ given, int limit,
@@ -378,40 +410,48 @@ head_join_kernel(const __grid_constant__ HeadPlan plan, const Mass* __restrict__
   const int row = blockIdx.x, lane = threadIdx.x;
   const int token = tokens[row];
   const float logit = token >= 0 && token < limit ? given[row] : __uint_as_float(0x7fc00000u);
-  int band = 0, block = row >> 8;
+  int band = 0, block = row / plan.block_rows;
   while (band + 1 < plan.bands && block >= plan.first[band + 1]) ++band;
   block -= plan.first[band];
   const int strips = plan.strips[band];
-  const size_t part = plan.part0[band] + ((size_t)block * 256 + (row & 255)) * strips;
+  const size_t part = plan.part0[band] + ((size_t)block * plan.block_rows + row % plan.block_rows) * strips;
   for (int i = lane; i < strips * top; i += 32) sh_keys[i] = keys[part * top + i];
-  Mass v = mass_none();
+  Mass v[HS_STRIPS / 32];
+  float most = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < HS_PAIRS / 32; ++i)
-    if (lane + 32 * i < strips) v = mass_join(v, mass[part + lane + 32 * i]);
-  v = mass_warp(v);
+  for (int i = 0; i < HS_STRIPS / 32; ++i) {
+    v[i] = lane + 32 * i < strips ? mass[part + lane + 32 * i] : mass_none();
+    most = fmaxf(most, v[i].m);
+  }
+  most = warp_max(most);
+  Mass all = {most, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < HS_STRIPS / 32; ++i) {
+    const Mass p = mass_over(v[i], most);
+    all.s += p.s, all.t += p.t;
+  }
+  all.s = warp_sum(all.s);
+  all.t = warp_sum(all.t);
   __syncwarp();
   TopKey mine = 0;
   if (top > 0) {
-    int head[HS_PAIRS / 32];
-    TopKey next[HS_PAIRS / 32];
+    int head[HS_STRIPS / 32];
+    TopKey next[HS_STRIPS / 32];
 #pragma unroll
-    for (int i = 0; i < HS_PAIRS / 32; ++i) {
+    for (int i = 0; i < HS_STRIPS / 32; ++i) {
       head[i] = (lane + 32 * i) * top;
       next[i] = lane + 32 * i < strips ? sh_keys[head[i]] : 0;
     }
     for (int j = 0; j < top; ++j) {
       TopKey best = 0;
 #pragma unroll
-      for (int i = 0; i < HS_PAIRS / 32; ++i)
+      for (int i = 0; i < HS_STRIPS / 32; ++i)
         if (next[i] > best) best = next[i];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const TopKey c = __shfl_xor_sync(0xffffffffu, best, o);
-        if (c > best) best = c;
-      }
+      const uint32_t place = (uint32_t)(best >> 32), first = __reduce_max_sync(0xffffffffu, place);
+      best = (TopKey)first << 32 | __reduce_max_sync(0xffffffffu, place == first ? (uint32_t)best : 0u);
       if (best == 0) break;
 #pragma unroll
-      for (int i = 0; i < HS_PAIRS / 32; ++i)
+      for (int i = 0; i < HS_STRIPS / 32; ++i)
         if (next[i] == best) {
           ++head[i];
           next[i] = head[i] < (lane + 32 * i + 1) * top ? sh_keys[head[i]] : 0;
@@ -419,30 +459,32 @@ head_join_kernel(const __grid_constant__ HeadPlan plan, const Mass* __restrict__
       if (lane == j) mine = best;
     }
   }
-  finish_row(v, logit, mine, top, row, out);
+  finish_row(all, logit, mine, top, row, out);
 }
 
-typedef void (*HeadKernel)(CUtensorMap, CUtensorMap, HeadPlan, int, int, int, float, float, const int*, int,
-                           float*, Mass*, TopKey*, int*);
+typedef void (*HeadKernel)(CUtensorMap, CUtensorMap, HeadPlan, int, int, int, float, float, const int*, int, float*,
+                           Mass*, TopKey*, int*);
 // The kernel whose lists have room for `top` keys
 #define HS_FORMS 9
 static int head_form(int top) { return (top + 3) / 4; }
-static HeadKernel head_kernel(int form) {
-  static const HeadKernel kernels[HS_FORMS] = {
-      head_scores_kernel<0>,  head_scores_kernel<4>,  head_scores_kernel<8>,  head_scores_kernel<12>, head_scores_kernel<16>,
-      head_scores_kernel<20>, head_scores_kernel<24>, head_scores_kernel<28>, head_scores_kernel<32>};
-  return kernels[form];
+#define HS_ALL(PAIR_)                                                                                    \
+  {head_scores_kernel<0, PAIR_>,  head_scores_kernel<4, PAIR_>,  head_scores_kernel<8, PAIR_>,           \
+   head_scores_kernel<12, PAIR_>, head_scores_kernel<16, PAIR_>, head_scores_kernel<20, PAIR_>,          \
+   head_scores_kernel<24, PAIR_>, head_scores_kernel<28, PAIR_>, head_scores_kernel<32, PAIR_>}
+static HeadKernel head_kernel(bool pair, int form) {
+  static const HeadKernel kernels[2][HS_FORMS] = {HS_ALL(false), HS_ALL(true)};
+  return kernels[pair][form];
 }
-static cudaError_t allow_smem(int form) {
-  static unsigned long long done[HS_FORMS] = {};
-  return mb_allow_smem((const void*)head_kernel(form), HS_SMEM, &done[form]);
+static cudaError_t allow_smem(bool pair, int form) {
+  static unsigned long long done[2][HS_FORMS] = {};
+  return mb_allow_smem((const void*)head_kernel(pair, form), HS_SMEM, &done[pair][form]);
 }
 
 // How many CTA pairs the device runs at once (0: the kernel cannot run here)
 static int head_pairs(int sms) {
   static int pairs = -1;
   if (pairs >= 0) return pairs;
-  if (allow_smem(HS_FORMS - 1) != cudaSuccess) {
+  if (allow_smem(true, HS_FORMS - 1) != cudaSuccess) {
     cudaGetLastError();
     return pairs = 0;
   }
@@ -458,53 +500,65 @@ static int head_pairs(int sms) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, head_kernel(HS_FORMS - 1), &cfg) != cudaSuccess) {
+  if (cudaOccupancyMaxActiveClusters(&n, head_kernel(true, HS_FORMS - 1), &cfg) != cudaSuccess) {
     cudaGetLastError();
     n = 0;
   }
   n = n > sms / 2 ? sms / 2 : n;
-  return pairs = n > HS_PAIRS ? HS_PAIRS : n;
+  return pairs = n > HS_STRIPS ? HS_STRIPS : n;
 }
 
-// Ids of a strip where `blocks` row blocks share the pairs, a multiple of 16
-static int strip_width(int blocks, int pairs, int limit) {
-  const int strips = pairs / blocks;
+// Pairs, or CTAs by themselves for rows that one of them holds: half of a pair's tile would be empty, and
+// its products take as long as the weights' way from memory. 5 and 20 alternatives, us in pairs and by themselves:
+// 128 rows of 512 values 71 105 | 50 85, of 1,024 75 110 | 69 95, of 2,048 120 147 | 124 144, of 4,096
+// 231 245 | 234 246.
+static bool in_pairs(int rows) { return rows > block_rows_of(false); }
+static int head_units(bool pair, int sms) {
+  const int pairs = head_pairs(sms);
+  return pair || pairs == 0 ? pairs : sms < HS_STRIPS ? sms : HS_STRIPS;
+}
+
+// Ids of a strip where `blocks` row blocks share the pairs (or CTAs), a multiple of 16
+static int strip_width(int blocks, int units, int limit) {
+  const int strips = units / blocks;
   return ((limit + strips - 1) / strips + 15) & ~15;
 }
 
-// Cuts `blocks` row blocks into bands of at most `pairs` blocks such that the strips' widths add up
+// Cuts a launch's row blocks into bands of at most `units` blocks such that the strips' widths add up
 // to the least: the time of a band is that of its widest strip, and a strip's start and end (its first tile
 // has nothing to overlap, its last one's values neither), which count as 512 ids. With 64 the 2,048 rows
 // above took four bands of two blocks, which fill the pairs exactly and read the weights four times: 2,090 us
 // where one band of eight takes 1,885, with 1,024 values 623 and 475.
-static void plan_bands(HeadPlan& plan, int blocks, int pairs, int limit) {
+static void plan_bands(HeadPlan& plan, int rows, int units, int limit) {
+  plan.block_rows = block_rows_of(in_pairs(rows));
+  const int blocks = (rows + plan.block_rows - 1) / plan.block_rows;
   int best[HS_BLOCKS + 1], take[HS_BLOCKS + 1];
   best[0] = 0;
   for (int n = 1; n <= blocks; ++n) {
     best[n] = 0x7fffffff;
-    for (int b = 1; b <= n && b <= pairs; ++b) {
-      const int cost = best[n - b] + strip_width(b, pairs, limit) + 512;
+    for (int b = 1; b <= n && b <= units; ++b) {
+      const int cost = best[n - b] + strip_width(b, units, limit) + 512;
       if (cost < best[n]) best[n] = cost, take[n] = b;
     }
   }
   plan.bands = 0;
   int first = 0, part = 0;
   for (int n = blocks; n > 0; n -= take[n]) {
-    const int i = plan.bands++, b = take[n], width = strip_width(b, pairs, limit);
+    const int i = plan.bands++, b = take[n], width = strip_width(b, units, limit);
     plan.first[i] = first;
     plan.blocks[i] = b;
     plan.width[i] = width;
     plan.strips[i] = (limit + width - 1) / width;
-    const int tiles = (width + 255) / 256;
+    const int tiles = (width + plan.block_rows - 1) / plan.block_rows;
     plan.tile[i] = ((width + tiles - 1) / tiles + 15) & ~15;
     plan.part0[i] = part;
     first += b;
-    part += b * 256 * plan.strips[i];
+    part += b * plan.block_rows * plan.strips[i];
   }
 }
 static int parts_of(const HeadPlan& plan) {
   const int i = plan.bands - 1;
-  return plan.part0[i] + plan.blocks[i] * 256 * plan.strips[i];
+  return plan.part0[i] + plan.blocks[i] * plan.block_rows * plan.strips[i];
 }
 
 // Whether mb_head_scores takes operands of these sizes and alignments on this device.
@@ -516,13 +570,13 @@ MB_EXPORT int mb_head_scores_supported(const void* A, int lda, const void* W, in
 // bytes of scratch that mb_head_scores needs: what the larger of its two plans takes (that of whole
 // launches, and that of the last one, which may be cut into more strips)
 MB_EXPORT long long mb_head_scores_scratch(int rows, int limit, int top, int sms) {
-  const int pairs = head_pairs(sms), most = HS_BLOCKS * 256;
-  if (pairs <= 0 || rows <= 0 || limit <= 0) return 0;
+  const int most = HS_BLOCKS * block_rows_of(true);
+  if (head_pairs(sms) <= 0 || rows <= 0 || limit <= 0) return 0;
   long long parts = 0;
   for (const int n : {rows < most ? 0 : most, rows % most}) {
     if (n == 0) continue;
     HeadPlan plan;
-    plan_bands(plan, (n + 255) / 256, pairs, limit);
+    plan_bands(plan, n, head_units(in_pairs(n), sms), limit);
     if (parts_of(plan) > parts) parts = parts_of(plan);
   }
   return parts * (12 + 8 * top) + 4ll * (rows < most ? rows : most) + 16;
@@ -542,19 +596,20 @@ MB_EXPORT int mb_head_scores(const void* A, int lda, const void* W, int rows, in
     MB_FAIL("mb_head_scores: rows of %d values, %d apart, are not taken", K, lda);
   if (scratch_bytes < mb_head_scores_scratch(rows, limit, top, sms))
     MB_FAIL("mb_head_scores: %lld bytes of scratch", scratch_bytes);
-  const int pairs = head_pairs(sms);
-  const int form = head_form(top);
-  if (cudaError_t e = allow_smem(form)) MB_FAIL("mb_head_scores: %s", cudaGetErrorString(e));
+  const int form = head_form(top), most = HS_BLOCKS * block_rows_of(true);
   cudaStream_t s = (cudaStream_t)stream;
   CUtensorMap tmB;
   if (!mb_make_map_bf16(&tmB, W, limit, K, K, 128, "mb_head_scores weight")) return -1;
-  for (int r0 = 0; r0 < rows; r0 += HS_BLOCKS * 256) {
-    const int n = rows - r0 < HS_BLOCKS * 256 ? rows - r0 : HS_BLOCKS * 256;
+  for (int r0 = 0; r0 < rows; r0 += most) {
+    const int n = rows - r0 < most ? rows - r0 : most;
+    const bool pair = in_pairs(n);
+    if (cudaError_t e = allow_smem(pair, form)) MB_FAIL("mb_head_scores: %s", cudaGetErrorString(e));
     const __nv_bfloat16* a = (const __nv_bfloat16*)A + (size_t)r0 * lda;
     HeadPlan plan = {};
-    plan_bands(plan, (n + 255) / 256, pairs, limit);
+    plan_bands(plan, n, head_units(pair, sms), limit);
     CUtensorMap tmA;
-    if (!mb_make_map_bf16(&tmA, a, n, K, lda, 128, "mb_head_scores input")) return -1;
+    const int box = pair ? box_rows<true>(n) : box_rows<false>(n);
+    if (!mb_make_map_bf16(&tmA, a, n, K, lda, box, "mb_head_scores input")) return -1;
     const size_t parts = parts_of(plan);
     TopKey* keys = (TopKey*)scratch;
     Mass* mass = (Mass*)(keys + parts * top);
@@ -562,9 +617,13 @@ MB_EXPORT int mb_head_scores(const void* A, int lda, const void* W, int rows, in
     int used = 0;
     for (int i = 0; i < plan.bands; ++i)
       if (plan.blocks[i] * plan.strips[i] > used) used = plan.blocks[i] * plan.strips[i];
-    cudaError_t e = mb_launch_clusters(head_kernel(form), dim3(2 * used), dim3(HS_THREADS), HS_SMEM, s,
-                                       2, tmA, tmB, plan, n, limit, K, scale, cap, tokens + r0, top,
-                                       given, mass, keys, error);
+    const dim3 block(HS_THREADS);
+    cudaError_t e =
+        pair ? mb_launch_clusters(head_kernel(true, form), dim3(2 * used), block, HS_SMEM, s, 2, tmA, tmB,
+                                  plan, n, limit, K, scale, cap, tokens + r0, top, given, mass, keys,
+                                  error)
+             : mb_launch(head_kernel(false, form), dim3(used), block, HS_SMEM, s, tmA, tmB, plan, n, limit,
+                         K, scale, cap, tokens + r0, top, given, mass, keys, error);
     if (e != cudaSuccess) MB_FAIL("mb_head_scores: %s", cudaGetErrorString(e));
     const ScoreOut out = {logprobs + r0, entropy + r0, top_ids + (size_t)r0 * top,
                           top_logprobs + (size_t)r0 * top};

@@ -19,13 +19,16 @@ from .linear import Linear, Pending
 SCORE_BAND = 1 << 28
 
 
-def scores_through_memory(rows: int, width: int, top: int) -> bool:
-    """Whether the logits of so few rows are better stored: the product of few rows streams the head
-    faster, while a strip of the fused kernel pays for its first tile and its lists. 151,936 ids, us
-    fused | stored, with 5 alternatives: 16 rows of 1,024 values 86 | 70, 48 rows 83 | 77, 64 rows 75 | 80,
-    32 rows of 2,048 114 | 115, 48 rows of 4,096 224 | 233; with 20: 128 rows of 512 105 | 79, of 1,024
-    111 | 109, 64 rows of 2,048 148 | 139, of 4,096 232 | 261."""
-    return rows <= 32 or rows * width <= (49152 if top <= 8 else 131072)
+def scores_through_memory(rows: int, width: int, vocab: int, top: int) -> bool:
+    """Whether the logits of these rows are better stored. Of few wide rows: the product of few rows
+    streams the head a little faster (1 row of 2,560 values before 151,936 ids 143 us against 154, 32 rows
+    150 against 154). Of many alternatives: the fused kernel keeps lists of its own for every strip
+    of a row, while the stored logits of few rows are read from L2. Fused | stored, us: 20 alternatives of
+    151,936 ids, 32 rows of 1,024 values 100 | 86, 96 rows 101 | 111; of 32,000 ids, 257 rows 73 | 57, 512
+    rows 80 | 70, 1,001 rows 109 | 117; 32 alternatives of 151,936, 128 rows 127 | 115, 256 rows 172 | 164,
+    of 2,560 values 205 | 248. With 8 or fewer the fused kernel is as quick from the first row on: 5
+    alternatives, 8 rows of 1,024 values 83 | 84, 128 rows 86 | 109."""
+    return (rows <= 32 and width >= 2048) or rows * vocab <= (top - 8) << 20
 
 
 class TokenEmbedding(Part):
@@ -100,7 +103,7 @@ class LmHead(Part):
         if rows == 0:
             return out
         tokens = tokens.contiguous()
-        if (self.linear.fast is not None and not scores_through_memory(rows, self.hidden, top)
+        if (self.linear.fast is not None and not scores_through_memory(rows, self.hidden, limit, top)
                 and K.head_scores_supported(h, weight)):
             K.head_scores(h, weight, limit, self.scale, self.softcap, tokens, top, out, rt.error_word)
             return out
