@@ -75,6 +75,12 @@ struct HeadWalk {
   __device__ __forceinline__ void step() { n += plan.tile[band]; }
 };
 
+// Notes of a row with lists of N places. Its strips share them: each leaves the greatest of its ids so far,
+// of four groups apart, in notes of its own or, as a maximum, in some that others use too. Whatever is there, the
+// greatest values of as many groups of ids, the `top`-th of them has `top` ids that are no less: no strip needs
+// what is below it, and when a strip looks does not show in the results.
+__host__ __device__ constexpr int notes_of(int n) { return n <= 8 ? 16 : n <= 16 ? 32 : 64; }
+
 // A row's greatest values so far, in order, in registers: the last `top` of N places (what stands above
 // them is never passed). A value goes in where it is greater, so the first of equals stays ahead.
 template <int N> struct TopList {
@@ -91,6 +97,7 @@ template <int N> struct TopList {
   }
   // One of many groups' greatest values: in the end the least of v is below no more than top - 1 groups
   __device__ __forceinline__ void probe(float x) {
+    x = fmaxf(x, -INFINITY);      // of nothing but NaN: none
 #pragma unroll
     for (int k = N - 1; k > 0; --k) v[k] = fmaxf(v[k], fminf(v[k - 1], x));
     v[0] = fmaxf(v[0], x);
@@ -99,7 +106,32 @@ template <int N> struct TopList {
   __device__ __forceinline__ void start(int top) {
     const float least = v[N - 1];
     clear(top);
-    if (least > -INFINITY) bar = least - 1e-6f * fabsf(least) - 1e-30f;
+    raise(least);
+  }
+  __device__ __forceinline__ void raise(float least) {
+    least = fminf(least, 3e38f);
+    if (least > -INFINITY) bar = fmaxf(bar, least - 1e-6f * fabsf(least) - 1e-30f);
+  }
+  // A bar from the row's notes (0: none yet)
+  __device__ __forceinline__ void look(const uint32_t* notes, int top) {
+    float u[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) u[k] = k < N - top ? INFINITY : -INFINITY;
+#pragma unroll
+    for (int j0 = 0; j0 < notes_of(N); j0 += 16) {
+      uint32_t place[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(place[j]) : "l"(notes + (j0 + j) * 256) : "memory");
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float x = place[j] == 0 ? -INFINITY : key_value((TopKey)place[j] << 32);
+#pragma unroll
+        for (int k = N - 1; k > 0; --k) u[k] = fmaxf(u[k], fminf(u[k - 1], x));
+        u[0] = fmaxf(u[0], x);
+      }
+    }
+    raise(u[N - 1]);
   }
   __device__ __forceinline__ void hush() { bar = INFINITY; }      // a row that is not there
   __device__ __forceinline__ void offer(float x, int i) {
@@ -126,6 +158,7 @@ template <> struct TopList<0> {
   __device__ __forceinline__ void clear(int) {}
   __device__ __forceinline__ void probe(float) {}
   __device__ __forceinline__ void start(int) {}
+  __device__ __forceinline__ void look(const uint32_t*, int) {}
   __device__ __forceinline__ void hush() {}
   __device__ __forceinline__ void offer(float, int) {}
   __device__ __forceinline__ void write(TopKey*, int) const {}
@@ -174,11 +207,14 @@ __device__ __forceinline__ void shape32(float* x, float scale, float cap) {
     }
   }
 }
-__device__ __forceinline__ float max32(const float* x) {
-  float m[4] = {x[0], x[1], x[2], x[3]};
+// The greatest of each eight
+__device__ __forceinline__ void max_eights(const float* x, float* m) {
 #pragma unroll
-  for (int j = 4; j < 32; ++j) m[j & 3] = fmaxf(m[j & 3], x[j]);
-  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+  for (int g = 0; g < 4; ++g) {
+    m[g] = x[8 * g];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) m[g] = fmaxf(m[g], x[8 * g + j]);
+  }
 }
 
 // Rows that are copied for a tile of `rows`: by pairs all, those beyond the last one as zeros; by a CTA by itself
@@ -194,7 +230,7 @@ __global__ void __launch_bounds__(HS_THREADS, 1)
 head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ HeadPlan plan, int rows, int limit, int K, float scale, float cap,
                    const int* __restrict__ tokens, int top, float* __restrict__ given, Mass* __restrict__ mass,
-                   TopKey* __restrict__ keys, int* __restrict__ error) {
+                   TopKey* __restrict__ keys, uint32_t* notes, int* __restrict__ error) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -298,34 +334,60 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       float m = -INFINITY, s = 0.f, t = 0.f;     // the row's mass
       TopList<N> list;
       list.clear(top);
-      bool fresh = true;
+      int seen = 0;                              // tiles of the strip
+      float groups[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // the greatest of every fourth eight
+      uint32_t* noted = nullptr;
+      if (PAIR && notes != nullptr) noted = notes + (size_t)(row >> 8) * (256 * notes_of(N)) + (row & 255);
+      auto note = [&]() {
+        if (noted == nullptr || row >= rows) return;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          asm volatile("red.relaxed.gpu.global.max.u32 [%0], %1;"
+                       ::"l"(noted + (walk.strip * 4 + g) % notes_of(N) * 256), "r"(key_place(groups[g]))
+                       : "memory");
+      };
       if (row >= rows) list.hush();
       const bool idle = walk.row0() + (int)rank * 128 + q * 32 >= rows;    // none of the warp's rows is there
       for (; walk.n < walk.end; walk.step(), ++it) {
         const int b = it & 1, cols = walk.cols();
+        // looked at after 1, 2, 4, ... tiles, while the next one is multiplied
+        if (PAIR && N > 0 && !idle && seen != 0 && noted != nullptr && (seen & (seen - 1)) == 0) {
+          if (row < rows) list.look(noted, top);
+          __syncwarp();
+        }
         mbar_wait(acc_full0 + 8 * b, (it >> 1) & 1, error, 64);
         tc_fence_after_sync();
         float tile_s = 0.f, tile_t = 0.f;        // the tile's part, over the same maximum
         const uint32_t taddr = tmem + b * 256 + ((uint32_t)(q * 32) << 16);
-        if (N > 0 && fresh && !idle) {
-          // A strip's first tile is read ahead for a bar: the `top`-th of its eights' greatest values. Without
-          // it the first values of all rows pass, one after another.
-          fresh = false;
+        if (N > 0 && !idle && seen == 0) {
+          // A strip's first tile is read ahead for a bar: the `top`-th of its eights' greatest values, or of its
+          // fours' where the eights are few (8 rows of 512 values, 20 alternatives of 32,000 ids: 35 us, 31 so).
+          // Without it the first values of all rows pass, one after another.
 #pragma unroll 1
           for (int c = 0; c < cols; c += 32) {
             float x[32];
             load32(taddr + c, x);
             if (shaped) shape32(x, scale, cap);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              float m = x[8 * g];
+            for (int g = 0; g < 8; g += 2) {
+              float four[2];
 #pragma unroll
-              for (int j = 1; j < 8; ++j) m = fmaxf(m, x[8 * g + j]);
-              if (c + 8 * g + 8 <= cols) list.probe(m);
+              for (int e = 0; e < 2; ++e)
+                four[e] = fmaxf(fmaxf(x[4 * (g + e)], x[4 * (g + e) + 1]),
+                                fmaxf(x[4 * (g + e) + 2], x[4 * (g + e) + 3]));
+              if (c + 4 * g + 8 > cols) continue;
+              groups[g >> 1] = fmaxf(groups[g >> 1], fmaxf(four[0], four[1]));
+              if (N <= 8 || cols >= 16 * top) {
+                list.probe(fmaxf(four[0], four[1]));
+              } else {
+                list.probe(four[0]);
+                list.probe(four[1]);
+              }
             }
           }
           list.start(top);
           if (row >= rows) list.hush();
+          if (PAIR) note();
         }
 #pragma unroll 1
         for (int c = 0; c < (idle ? 0 : cols); c += 32) {
@@ -338,7 +400,13 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             for (int j = 0; j < 32; ++j)
               if (j >= n) x[j] = -INFINITY;
           }
-          const float most = max32(x);
+          float eights[4];
+          max_eights(x, eights);
+          const float most = fmaxf(fmaxf(eights[0], eights[1]), fmaxf(eights[2], eights[3]));
+          if (PAIR && N > 0 && noted != nullptr) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) groups[g] = fmaxf(groups[g], eights[g]);
+          }
           if (most > m) {
             const Mass row_part = mass_over({m, s, t}, most), tile_part = mass_over({m, tile_s, tile_t}, most);
             m = most;
@@ -374,6 +442,8 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         }
         s += tile_s;
         t += tile_t;
+        ++seen;
+        if (PAIR && N > 0 && !idle && (seen & (seen - 1)) == 0) note();
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) {
@@ -415,7 +485,9 @@ head_join_kernel(const __grid_constant__ HeadPlan plan, const Mass* __restrict__
   block -= plan.first[band];
   const int strips = plan.strips[band];
   const size_t part = plan.part0[band] + ((size_t)block * plan.block_rows + row % plan.block_rows) * strips;
-  for (int i = lane; i < strips * top; i += 32) sh_keys[i] = keys[part * top + i];
+  for (int i = lane; i < strips * top; i += 32)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(sh_keys + i)), "l"(keys + part * top + i)
+                 : "memory");
   Mass v[HS_STRIPS / 32];
   float most = -INFINITY;
 #pragma unroll
@@ -432,38 +504,44 @@ head_join_kernel(const __grid_constant__ HeadPlan plan, const Mass* __restrict__
   }
   all.s = warp_sum(all.s);
   all.t = warp_sum(all.t);
+  asm volatile("cp.async.wait_all;" ::: "memory");
   __syncwarp();
   TopKey mine = 0;
   if (top > 0) {
     int head[HS_STRIPS / 32];
-    TopKey next[HS_STRIPS / 32];
+    TopKey next[HS_STRIPS / 32], first = 0;      // of the lane's strips, and the greatest of those
 #pragma unroll
     for (int i = 0; i < HS_STRIPS / 32; ++i) {
       head[i] = (lane + 32 * i) * top;
       next[i] = lane + 32 * i < strips ? sh_keys[head[i]] : 0;
+      if (next[i] > first) first = next[i];
     }
     for (int j = 0; j < top; ++j) {
-      TopKey best = 0;
+      const uint32_t place = (uint32_t)(first >> 32), best = __reduce_max_sync(0xffffffffu, place);
+      const uint32_t id = __reduce_max_sync(0xffffffffu, place == best ? (uint32_t)first : 0u);
+      if (id == 0) break;
+      const TopKey key = (TopKey)best << 32 | id;
+      if (lane == j) mine = key;
+      if (first == key) {
+        first = 0;
 #pragma unroll
-      for (int i = 0; i < HS_STRIPS / 32; ++i)
-        if (next[i] > best) best = next[i];
-      const uint32_t place = (uint32_t)(best >> 32), first = __reduce_max_sync(0xffffffffu, place);
-      best = (TopKey)first << 32 | __reduce_max_sync(0xffffffffu, place == first ? (uint32_t)best : 0u);
-      if (best == 0) break;
-#pragma unroll
-      for (int i = 0; i < HS_STRIPS / 32; ++i)
-        if (next[i] == best) {
-          ++head[i];
-          next[i] = head[i] < (lane + 32 * i + 1) * top ? sh_keys[head[i]] : 0;
+        for (int i = 0; i < HS_STRIPS / 32; ++i) {
+          if (32 * i >= strips) break;
+          if (next[i] == key) {
+            ++head[i];
+            next[i] = head[i] < (lane + 32 * i + 1) * top ? sh_keys[head[i]] : 0;
+          }
+          if (next[i] > first) first = next[i];
         }
-      if (lane == j) mine = best;
+      }
+      __syncwarp();
     }
   }
   finish_row(all, logit, mine, top, row, out);
 }
 
 typedef void (*HeadKernel)(CUtensorMap, CUtensorMap, HeadPlan, int, int, int, float, float, const int*, int, float*,
-                           Mass*, TopKey*, int*);
+                           Mass*, TopKey*, uint32_t*, int*);
 // The kernel whose lists have room for `top` keys
 #define HS_FORMS 9
 static int head_form(int top) { return (top + 3) / 4; }
@@ -556,6 +634,17 @@ static void plan_bands(HeadPlan& plan, int rows, int units, int limit) {
     part += b * plan.block_rows * plan.strips[i];
   }
 }
+// Whether a row's strips are wide enough that what they note pays for a memset ahead of the kernel. 5 and 20
+// alternatives, us without and with notes: strips of 4,106 ids (333 rows of 512 values, 151,936 ids) 105 155 |
+// 94 145, of 8,450 (1,001 rows) 184 254 | 172 234, the same of 1,024 values 239 | 228; of 3,556 (2,048 rows of
+// 1,024 values, 32,000 ids) 107 146 | 105 147. CTAs by themselves have narrower ones (8 rows of 1,024
+// values, 151,936 ids 57 77 | 58 89).
+static bool notes_pay(const HeadPlan& plan, bool pair, int top) {
+  int width = 0;
+  for (int i = 0; i < plan.bands; ++i) width = plan.width[i] > width ? plan.width[i] : width;
+  return pair && top > 0 && width >= 4096;
+}
+static long long notes_bytes(int rows, int form) { return (rows + 255ll) / 256 * 1024 * notes_of(4 * form); }
 static int parts_of(const HeadPlan& plan) {
   const int i = plan.bands - 1;
   return plan.part0[i] + plan.blocks[i] * plan.block_rows * plan.strips[i];
@@ -579,7 +668,8 @@ MB_EXPORT long long mb_head_scores_scratch(int rows, int limit, int top, int sms
     plan_bands(plan, n, head_units(in_pairs(n), sms), limit);
     if (parts_of(plan) > parts) parts = parts_of(plan);
   }
-  return parts * (12 + 8 * top) + 4ll * (rows < most ? rows : most) + 16;
+  const int one = rows < most ? rows : most;
+  return parts * (12 + 8 * top) + 4ll * one + (top > 0 ? notes_bytes(one, head_form(top)) : 0) + 16;
 }
 
 // For rows A [rows, K] (bfloat16, `lda` values from row to row) and a head W [V, K]: the scores of
@@ -614,6 +704,10 @@ MB_EXPORT int mb_head_scores(const void* A, int lda, const void* W, int rows, in
     TopKey* keys = (TopKey*)scratch;
     Mass* mass = (Mass*)(keys + parts * top);
     float* given = (float*)(mass + parts);
+    uint32_t* notes = notes_pay(plan, pair, top) ? (uint32_t*)(given + n) : nullptr;
+    if (notes != nullptr)
+      if (cudaError_t e = cudaMemsetAsync(notes, 0, notes_bytes(n, form), s))
+        MB_FAIL("mb_head_scores: %s", cudaGetErrorString(e));
     int used = 0;
     for (int i = 0; i < plan.bands; ++i)
       if (plan.blocks[i] * plan.strips[i] > used) used = plan.blocks[i] * plan.strips[i];
@@ -621,9 +715,9 @@ MB_EXPORT int mb_head_scores(const void* A, int lda, const void* W, int rows, in
     cudaError_t e =
         pair ? mb_launch_clusters(head_kernel(true, form), dim3(2 * used), block, HS_SMEM, s, 2, tmA, tmB,
                                   plan, n, limit, K, scale, cap, tokens + r0, top, given, mass, keys,
-                                  error)
+                                  notes, error)
              : mb_launch(head_kernel(false, form), dim3(used), block, HS_SMEM, s, tmA, tmB, plan, n, limit,
-                         K, scale, cap, tokens + r0, top, given, mass, keys, error);
+                         K, scale, cap, tokens + r0, top, given, mass, keys, notes, error);
     if (e != cudaSuccess) MB_FAIL("mb_head_scores: %s", cudaGetErrorString(e));
     const ScoreOut out = {logprobs + r0, entropy + r0, top_ids + (size_t)r0 * top,
                           top_logprobs + (size_t)r0 * top};

@@ -269,6 +269,27 @@ def test_head_broken_rows(form, rows):
         assert torch.equal(a[~bad], b[~bad])
 
 
+@pytest.mark.parametrize("rows,V,top", [(140, 304003, 5), (260, 160001, 20), (150, 310000, 32)])
+def test_head_wide_strips(form, rows, V, top):
+    """Strips of more than 4,096 ids, which tell one another what they have found: ids in rising and in falling
+    order (511 values, so most of them many times), all equal, the greatest in one place, and as they
+    come. When a strip looks must not show."""
+    h, w, tokens, dh, dw, dt = head_case(rows, V, 16, V, torch.bfloat16)
+    w[:, 0] = (np.arange(V) * 511 // V - 255) * 2.0 ** -9
+    w[:, 1] = 0.0
+    w[V // 3:V // 3 + 50, 1] = 0.25
+    h[0:4] = 0.0
+    h[1, 0], h[2, 0], h[3, 1] = 1.0, -1.0, 1.0
+    head = make_head(dw.copy_(torch.from_numpy(w)), torch.bfloat16)
+    dh.copy_(torch.from_numpy(h))
+    got = head.score(dh, dt, top)
+    head.linear.rt.check()
+    oracle.check(got, h @ w.T, tokens, top)
+    for _ in range(5):
+        for a, b in zip(head.score(dh, dt, top).tensors(), got.tensors()):
+            assert torch.equal(a, b)
+
+
 def test_bands_of_stored_rows(monkeypatch):
     """Rows that go through memory in several bands."""
     monkeypatch.setattr(embedding, "SCORE_BAND", 1)
