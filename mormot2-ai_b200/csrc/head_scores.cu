@@ -16,12 +16,13 @@
 // Bound: the tensor cores, from K of some 1,500 on (rows padded to 256; 151,936 ids, 5 alternatives: 1,024 rows of
 // 4,096 values 804 us with the tensor pipe 98 % active, weights read once, 1.30 GB; 2,048 rows again and
 // again 1.35 PFLOP/s under the power cap, on rows of few bits 1.53). Below that the four warps that read
-// tensor memory: some 550 cycles for 32 ids of a row (the exponentials alone take 256), and with 5 or 20
-// alternatives 280 or 700 more, most of them in the first tiles (1,024 values a row, 2,048 rows: 406, 475 and
-// 650 us). Up to 128 rows the head's bytes (1,024 values: 57 to 61 us, 5.1 to 5.4 TB/s; 4,096: 222, 5.6).
+// tensor memory: some 550 cycles for 32 ids of a row (the exponentials alone take 256), and the lists, some
+// 110 instructions a value that goes in (1,024 values a row, 1,001 rows: 212 us without alternatives, 228 with 5,
+// 300 with 20). Up to 128 rows the head's bytes (1,024 values: 57 to 61 us, 5.1 to 5.4 TB/s; 4,096: 222, 5.6).
 // Taken back: two such warps a quarter of the lanes, a tile each in turn (their lists see half the ids each,
 // and together nearly twice the new values: 501 us, 656 with 20); ids in a log beside the values in
-// registers (810 with 20: every value's way to the log is a branch); a CTA by itself with tiles of 256 ids
+// registers (810 with 20: every value's way to the log is a branch); values held back in shared memory, 16 a
+// row, and put in the lists by all rows at once (333 rows of 1,024 values with 20: 175 us against 172); a CTA by itself with tiles of 256 ids
 // (128 rows of 2,048 values 124 us against 115, of 4,096 242 against 223; four stages instead of six); pairs that
 // copy no rows beyond the last one (129 rows of 1,024 values 66 us against 64).
 #include "scores.cuh"
