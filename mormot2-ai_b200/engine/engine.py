@@ -304,9 +304,11 @@ class Engine:
                     raise InferError(f"slot {e.slot}: token {int(tokens[bad][0])} is outside "
                                      f"the vocabulary of {self.vocab_size}")
             if isinstance(e.want, np.ndarray):
-                want = e.want if len(tokens) > 1 else e.want.tolist()
-                outside = any(want) if len(tokens) == 1 else ( 
-                    want.size and not 0 <= want.min() <= want.max() < len(tokens))
+                # (64 bits: added to a first row, narrower integers would wrap)
+                want = e.want.astype(np.int64).reshape(-1)
+                outside = want.size and not 0 <= want.min() <= want.max() < len(tokens)
+                if len(tokens) == 1:
+                    want = want.tolist()
             else:
                 want = [len(tokens) - 1] if e.want is None else [int(w) for w in e.want]
                 outside = any(not 0 <= w < len(tokens) for w in want)

@@ -55,6 +55,26 @@ def test_score_is_what_the_logits_say(tiny, dtype, cut):
     oracle.check(got, x.numpy(), tokens, 7, 0.0 if dtype == "float32" else logits_off(eng))
 
 
+@pytest.mark.parametrize("kind", [np.int8, np.uint8, np.int16, np.int64, np.float64])
+def test_places_of_any_integer_type(tiny, kind):
+    """Places behind rows whose number the array's own type does not hold, and in a step of single tokens."""
+    eng = engine_of(tiny, "float32")
+    texts = [tiny.tokens(n, seed=n) for n in (100, 110, 120)]
+    slots = [eng.open() for _ in texts]
+    places = [7, 99, 3]
+    want = eng.step([Entry(s, t, places) for s, t in zip(slots, texts)]).clone()
+    alone = eng.step([Entry(slots[0], [5], [0, 0])]).clone()
+    for s in slots:
+        eng.truncate(s, 0)
+    got = eng.step([Entry(s, t, np.array(places, kind)) for s, t in zip(slots, texts)])
+    eng.rt.check()
+    assert (got == want).all()
+    assert (eng.step([Entry(slots[0], [5], np.array([0, 0], kind))]) == alone).all()
+    for bad in ([100, 0], [-1], [3, 300]):
+        with pytest.raises(InferError):
+            eng.step([Entry(slots[0], texts[0], np.array(bad, np.int16))])
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_score_token_by_token(tiny, dtype):
     """Decode passes: eager, captured, replayed; then a score of nothing."""
