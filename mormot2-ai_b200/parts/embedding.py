@@ -95,6 +95,8 @@ class LmHead(Part):
             with K.on_device_of(h):
                 return self.score(h, tokens, top, vocab_limit)
         rows, weight, rt = h.shape[0], self.linear.weight, self.linear.rt
+        if not self.hidden <= h.stride(0) < 1 << 31:      # one row many times, or rows 4 GiB apart
+            h = h.clone(memory_format=torch.contiguous_format)
         floats = h if h.dtype == torch.float32 else rt.workspace
         if floats is None:
             out = Scores.empty(rows, top, h.device)

@@ -253,6 +253,24 @@ def test_head_strides_limit_and_ties(form, rows):
     oracle.check(got, h @ w.T, tokens % 1501, 16)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_head_rows_anywhere(form, dtype):
+    """One row many times, a single row with a stride of nothing, and rows 2^32 + 64 values apart (a
+    stride that 32 bits would take for 64)."""
+    t = getattr(torch, dtype)
+    h, w, tokens, dh, dw, dt = head_case(150, 2000, 64, 37, t)
+    head = make_head(dw, t)
+    one = head.score(dh[:1].expand(150, 64), dt, 6)
+    oracle.check(one, np.repeat(h[:1], 150, 0) @ w.T, tokens, 6)
+    alone = head.score(dh[3].as_strided((1, 64), (1, 1)), dt[3:4], 6)
+    oracle.check(alone, h[3:4] @ w.T, tokens[3:4], 6)
+    apart = torch.empty(2 ** 32 + 128, dtype=t, device=DEV)
+    far = apart.as_strided((2, 64), (2 ** 32 + 64, 1))
+    far.copy_(dh[:2])
+    apart[64:128] = 7.0                 # where the second row would be
+    oracle.check(head.score(far, dt[:2], 6), h[:2] @ w.T, tokens[:2], 6)
+
+
 @pytest.mark.parametrize("rows", [6, 300])
 def test_head_broken_rows(form, rows):
     """A row with an infinity or a NaN has no distribution; its neighbours keep theirs."""
