@@ -1522,13 +1522,17 @@ def token_scores(logits: torch.Tensor, vocab: int, tokens: torch.Tensor, top: in
           out.top_logprobs.data_ptr(), _sms(), _stream())
 
 
+_HEAD_SCORES = [_addr, _i, _addr, _i, _i, _i, _f, _f, _addr, _i, _addr, _addr, _addr, _addr, _addr, _ll, _addr,
+                _i, _addr]
+
+
 def head_scores_supported(h: torch.Tensor, w: torch.Tensor) -> bool:
     """Whether ``head_scores`` takes these rows and this head."""
-    if h.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
+    if h.dtype is not torch.bfloat16 or w.dtype is not torch.bfloat16:
         return False
     f, _ = _functions.get("mb_head_scores_supported") or _function(
-        "head_scores", "mb_head_scores_supported", [_vp, _i, _vp, _i, _i])
-    return bool(f(_ptr(h), h.stride(0), _ptr(w), w.shape[1], _sms()))
+        "head_scores", "mb_head_scores_supported", [_addr, _i, _addr, _i, _i])
+    return f(h.data_ptr(), h.stride(0), w.data_ptr(), w.shape[1], _sms()) != 0
 
 
 def head_scores(h: torch.Tensor, w: torch.Tensor, limit: int, scale: float, cap: float,
@@ -1538,14 +1542,15 @@ def head_scores(h: torch.Tensor, w: torch.Tensor, limit: int, scale: float, cap:
     rows, Kd = h.shape
     assert w.shape[1] == Kd and h.stride(1) == 1 and 0 < limit <= w.shape[0]
     _contig(w, "the weight")
+    sms = _sms()
     f, _ = _functions.get("mb_head_scores_scratch") or _function(
         "head_scores", "mb_head_scores_scratch", [_i, _i, _i, _i], _ll)
-    scratch = torch.empty(f(rows, limit, top, _sms()), dtype=torch.uint8, device=h.device)
-    _call("head_scores", "mb_head_scores",
-          [_vp, _i, _vp, _i, _i, _i, _f, _f, _vp, _i, _vp, _vp, _vp, _vp, _vp, _ll, _vp, _i, _vp],
-          _ptr(h), h.stride(0), _ptr(w), rows, limit, Kd, float(scale), float(cap), _ptr(tokens),
-          top, _ptr(out.logprobs), _ptr(out.entropy), _ptr(out.top_ids), _ptr(out.top_logprobs),
-          _ptr(scratch), scratch.numel(), _ptr(error), _sms(), _stream(),
+    size = f(rows, limit, top, sms)
+    scratch = h.new_empty(size // 2 + 1)
+    _call("head_scores", "mb_head_scores", _HEAD_SCORES,
+          h.data_ptr(), h.stride(0), w.data_ptr(), rows, limit, Kd, scale, cap, tokens.data_ptr(),
+          top, out.logprobs.data_ptr(), out.entropy.data_ptr(), out.top_ids.data_ptr(),
+          out.top_logprobs.data_ptr(), scratch.data_ptr(), size, error.data_ptr(), sms, _stream(),
           launches=2 * -(-rows // 16384))
 
 
