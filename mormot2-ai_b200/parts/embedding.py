@@ -24,9 +24,9 @@ def scores_through_memory(rows: int, width: int, vocab: int, top: int) -> bool:
     streams the head a little faster (1 row of 2,560 values before 151,936 ids 143 us against 154, 32 rows
     150 against 154). Of many alternatives: the fused kernel keeps lists of its own for every strip
     of a row, while the stored logits of few rows are read from L2. Fused | stored, us: 20 alternatives of
-    151,936 ids, 32 rows of 1,024 values 100 | 86, 96 rows 101 | 111; of 32,000 ids, 257 rows 73 | 57, 512
-    rows 80 | 70, 1,001 rows 109 | 117; 32 alternatives of 151,936, 128 rows 127 | 115, 256 rows 172 | 164,
-    of 2,560 values 205 | 248. With 8 or fewer the fused kernel is as quick from the first row on: 5
+    151,936 ids, 32 rows of 1,024 values 93 | 88, 96 rows 94 | 113; of 32,000 ids, 257 rows 72 | 57, 512
+    rows 80 | 70, 1,001 rows 97 | 117; 32 alternatives of 151,936, 128 rows 129 | 117, 257 rows 201 | 201,
+    of 2,560 values 291 | 330. With 8 or fewer the fused kernel is as quick from the first row on: 5
     alternatives, 8 rows of 1,024 values 83 | 84, 128 rows 86 | 109."""
     return (rows <= 32 and width >= 2048) or rows * vocab <= (top - 8) << 20
 
