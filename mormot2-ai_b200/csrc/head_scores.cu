@@ -636,14 +636,14 @@ static void plan_bands(HeadPlan& plan, int rows, int units, int limit) {
   }
 }
 // Whether a row's strips are wide enough that what they note pays for a memset ahead of the kernel. 5 and 20
-// alternatives, us without and with notes: strips of 4,106 ids (333 rows of 512 values, 151,936 ids) 105 155 |
-// 94 145, of 8,450 (1,001 rows) 184 254 | 172 234, the same of 1,024 values 239 | 228; of 3,556 (2,048 rows of
-// 1,024 values, 32,000 ids) 107 146 | 105 147. CTAs by themselves have narrower ones (8 rows of 1,024
-// values, 151,936 ids 57 77 | 58 89).
+// alternatives, us without and with notes: 200 rows of 512 values, 151,936 ids (strips of 2,054) 69 107 | 63 104,
+// 1,001 rows (8,450) 184 254 | 172 234, 400 rows and 65,536 ids (1,772) 58 93 | 53 90; of 1,024 values the first
+// 77 113 | 75 109, the last 63 100 | 60 96. CTAs by themselves have narrower ones (8 rows of 1,024 values, 151,936
+// ids 57 77 | 58 89).
 static bool notes_pay(const HeadPlan& plan, bool pair, int top) {
   int width = 0;
   for (int i = 0; i < plan.bands; ++i) width = plan.width[i] > width ? plan.width[i] : width;
-  return pair && top > 0 && width >= 4096;
+  return pair && top > 0 && width >= 1024;
 }
 static long long notes_bytes(int rows, int form) { return (rows + 255ll) / 256 * 1024 * notes_of(4 * form); }
 static int parts_of(const HeadPlan& plan) {

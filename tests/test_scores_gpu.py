@@ -289,7 +289,7 @@ def test_head_broken_rows(form, rows):
 
 @pytest.mark.parametrize("rows,V,top", [(140, 304003, 5), (260, 160001, 20), (150, 310000, 32)])
 def test_head_wide_strips(form, rows, V, top):
-    """Strips of more than 4,096 ids, which tell one another what they have found: ids in rising and in falling
+    """Wide strips, which tell one another what they have found: ids in rising and in falling
     order (511 values, so most of them many times), all equal, the greatest in one place, and as they
     come. When a strip looks must not show."""
     h, w, tokens, dh, dw, dt = head_case(rows, V, 16, V, torch.bfloat16)
