@@ -18,12 +18,13 @@
 // again 1.35 PFLOP/s under the power cap, on rows of few bits 1.53). Below that the four warps that read
 // tensor memory: some 550 cycles for 32 ids of a row (the exponentials alone take 256), and the lists, some
 // 110 instructions a value that goes in (1,024 values a row, 1,001 rows: 212 us without alternatives, 228 with 5,
-// 300 with 20). Up to 128 rows the head's bytes (1,024 values: 57 to 61 us, 5.1 to 5.4 TB/s; 4,096: 222, 5.6).
+// 300 with 20). Up to 128 rows the head's bytes (24 rows of 1,024 values: 52 us, 6.0 TB/s; of 4,096:
+// 188, 6.6; 128 rows 55 and 214).
 // Taken back: two such warps a quarter of the lanes, a tile each in turn (their lists see half the ids each,
 // and together nearly twice the new values: 501 us, 656 with 20); ids in a log beside the values in
 // registers (810 with 20: every value's way to the log is a branch); values held back in shared memory, 16 a
-// row, and put in the lists by all rows at once (333 rows of 1,024 values with 20: 175 us against 172); a CTA by itself with tiles of 256 ids
-// (128 rows of 2,048 values 124 us against 115, of 4,096 242 against 223; four stages instead of six); pairs that
+// row, and put in the lists by all rows at once (333 rows of 1,024 values with 20: 175 us against 172); a CTA by
+// itself with tiles of 256 ids (128 rows of 2,048 values 124 us against 115, of 4,096 242 against 223); pairs that
 // copy no rows beyond the last one (129 rows of 1,024 values 66 us against 64).
 #include "scores.cuh"
 #include "tc_common.cuh"
@@ -35,11 +36,12 @@ MB_DEFINE_LAST_ERROR
 #define HS_THREADS 192
 #define HS_BK 64
 #define HS_HALF (128 * HS_BK * 2)            // 128 rows of an operand in a stage
-#define HS_STAGES 6
+#define HS_RING (12 * HS_HALF)               // of all stages
+#define HS_STAGES 12                         // at most
 #define HS_STRIPS 160                        // strips of a row at most
 #define HS_BLOCKS 64                         // row blocks of a launch at most
 #define HS_STAGED (4 * 32 * 128)             // 32 values of 32 rows for each epilogue warp
-#define HS_SMEM (1024 + HS_STAGES * 2 * HS_HALF + 256 + HS_STAGED)
+#define HS_SMEM (1024 + HS_RING + 256 + HS_STAGED)
 
 // A CTA pair multiplies 256 rows with 256 ids, each CTA bringing half of both; a CTA by itself 128 with 128.
 __host__ __device__ constexpr int block_rows_of(bool pair) { return pair ? 256 : 128; }
@@ -47,6 +49,7 @@ __host__ __device__ constexpr int block_rows_of(bool pair) { return pair ? 256 :
 // A band: `blocks` row blocks from `first` on, each in `strips` strips of `width` ids, tiles of `tile`
 struct HeadPlan {
   int bands, block_rows;
+  int box, stages;           // rows of the head that a CTA copies for a tile, and stages of the ring
   int first[HS_BLOCKS], blocks[HS_BLOCKS], strips[HS_BLOCKS], width[HS_BLOCKS], tile[HS_BLOCKS];
   int part0[HS_BLOCKS];      // where a band's parts begin: [block][row][strips]
 };
@@ -220,8 +223,9 @@ __device__ __forceinline__ void max_eights(const float* x, float* m) {
 
 // Rows that are copied for a tile of `rows`: by pairs all, those beyond the last one as zeros; by a CTA by itself
 // no more than are there, where the copies' zeros take longer than the weights (1,024 values a row: 4 rows
-// 82 us in a box of 128 rows, 61 in one of 8). Behind them the tile holds whatever was there; nobody reads
-// its products. Pairs multiply for longer than they copy, and zeros are what keeps the tensor cores coolest.
+// 82 us in a box of 128 rows, 61 in one of 8), and the stages lie that close together: up to 12 of them instead of
+// 6 (24 rows of 4,096 values 203 -> 188 us). Behind its rows a tile holds whatever is there; nobody reads the
+// products. Pairs multiply for longer than they copy, and zeros are what keeps the tensor cores coolest.
 template <bool PAIR> __host__ __device__ __forceinline__ int box_rows(int rows) {
   return PAIR ? 128 : (rows + 7) & ~7;
 }
@@ -235,8 +239,7 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
-  const uint32_t sA = base, sB = base + HS_STAGES * HS_HALF;
-  const uint32_t bars = base + HS_STAGES * 2 * HS_HALF;
+  const uint32_t bars = base + HS_RING;
   const uint32_t full0 = bars, empty0 = bars + 8 * HS_STAGES;
   const uint32_t acc_full0 = bars + 16 * HS_STAGES, acc_empty0 = acc_full0 + 16;
   const uint32_t slot = acc_empty0 + 16;
@@ -245,10 +248,12 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_rank() : 0;
   const int nkb = (K + HS_BK - 1) / HS_BK;
-  const int row_bytes = box_rows<PAIR>(rows) * HS_BK * 2;
+  const int row_bytes = box_rows<PAIR>(rows) * HS_BK * 2, id_bytes = (PAIR ? 128 : plan.box) * HS_BK * 2;
+  const int stages = PAIR ? HS_RING / (2 * HS_HALF) : plan.stages;
+  const uint32_t sA = base, sB = base + stages * row_bytes;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < HS_STAGES; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(full0 + 8 * s, 1);
       mbar_init(empty0 + 8 * s, 1);
     }
@@ -277,21 +282,21 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       while (walk.next_strip()) {
         const int m0 = walk.row0() + (int)rank * 128;
         for (; walk.n < walk.end; walk.step()) {
-          // each CTA of a pair holds half of the tile's ids (whole boxes of 128 are copied)
+          // each CTA of a pair holds half of the tile's ids (whole boxes are copied)
           const int n0 = walk.n + (int)rank * (((walk.cols() + 15) & ~15) >> 1);
           for (int i = 0; i < nkb; ++i) {
             mbar_wait(empty0 + 8 * s, ph ^ 1, error, 61);
             if (PAIR) {
-              if (rank == 0) mbar_expect_tx(full0 + 8 * s, 4 * HS_HALF);
+              if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * (row_bytes + id_bytes));
               const uint32_t full_lead = cluster_addr_of(full0 + 8 * s, 0);
-              tma_load_2d_pair(sA + s * HS_HALF, &tmA, i * HS_BK, m0, full_lead);
-              tma_load_2d_pair(sB + s * HS_HALF, &tmB, i * HS_BK, n0, full_lead);
+              tma_load_2d_pair(sA + s * row_bytes, &tmA, i * HS_BK, m0, full_lead);
+              tma_load_2d_pair(sB + s * id_bytes, &tmB, i * HS_BK, n0, full_lead);
             } else {
-              mbar_expect_tx(full0 + 8 * s, HS_HALF + row_bytes);
-              tma_load_2d(sA + s * HS_HALF, &tmA, i * HS_BK, m0, full0 + 8 * s);
-              tma_load_2d(sB + s * HS_HALF, &tmB, i * HS_BK, n0, full0 + 8 * s);
+              mbar_expect_tx(full0 + 8 * s, row_bytes + id_bytes);
+              tma_load_2d(sA + s * row_bytes, &tmA, i * HS_BK, m0, full0 + 8 * s);
+              tma_load_2d(sB + s * id_bytes, &tmB, i * HS_BK, n0, full0 + 8 * s);
             }
-            if (++s == HS_STAGES) { s = 0; ph ^= 1; }
+            if (++s == stages) { s = 0; ph ^= 1; }
           }
         }
       }
@@ -309,15 +314,15 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           for (int i = 0; i < nkb; ++i) {
             mbar_wait(full0 + 8 * s, ph, error, 63);
             tc_fence_after_sync();
-            const uint64_t da = umma_desc_k128(sA + s * HS_HALF);
-            const uint64_t db = umma_desc_k128(sB + s * HS_HALF);
+            const uint64_t da = umma_desc_k128(sA + s * row_bytes);
+            const uint64_t db = umma_desc_k128(sB + s * id_bytes);
 #pragma unroll
             for (int k = 0; k < HS_BK / 16; ++k) {
               if (PAIR) umma_bf16_pair(tmem + b * 256, da + 2 * k, db + 2 * k, idesc, (i | k) != 0);
               else umma_bf16(tmem + b * 256, da + 2 * k, db + 2 * k, idesc, (i | k) != 0);
             }
             if (PAIR) umma_commit_pair(empty0 + 8 * s, 3); else umma_commit(empty0 + 8 * s);
-            if (++s == HS_STAGES) { s = 0; ph ^= 1; }
+            if (++s == stages) { s = 0; ph ^= 1; }
           }
           if (PAIR) umma_commit_pair(acc_full0 + 8 * b, 3); else umma_commit(acc_full0 + 8 * b);
         }
@@ -603,12 +608,26 @@ static int strip_width(int blocks, int units, int limit) {
   return ((limit + strips - 1) / strips + 15) & ~15;
 }
 
+// Ids of a tile of a CTA by itself, a multiple of 16. All of a tile is copied, so it should not reach beyond the
+// strip: 24 rows of 4,096 values, strips of 1,040 ids, in tiles of 128 (1,152 copied) 208 us, of 96 (1,056) 188. A
+// tile itself costs as much as some 32,768 values of the head: of 512 values a row 31 and 36 us.
+static int tile_of(int width, int K) {
+  const int most = block_rows_of(false);
+  int best = most;
+  long long cost = 0;
+  for (int t = most; t >= 64; t -= 16) {
+    const long long c = (width + t - 1) / t * ((long long)t * K + 32768);
+    if (t == most || c < cost) best = t, cost = c;
+  }
+  return best;
+}
+
 // Cuts a launch's row blocks into bands of at most `units` blocks such that the strips' widths add up
 // to the least: the time of a band is that of its widest strip, and a strip's start and end (its first tile
 // has nothing to overlap, its last one's values neither), which count as 512 ids. With 64 the 2,048 rows
 // above took four bands of two blocks, which fill the pairs exactly and read the weights four times: 2,090 us
 // where one band of eight takes 1,885, with 1,024 values 623 and 475.
-static void plan_bands(HeadPlan& plan, int rows, int units, int limit) {
+static void plan_bands(HeadPlan& plan, int rows, int units, int limit, int K) {
   plan.block_rows = block_rows_of(in_pairs(rows));
   const int blocks = (rows + plan.block_rows - 1) / plan.block_rows;
   int best[HS_BLOCKS + 1], take[HS_BLOCKS + 1];
@@ -633,6 +652,12 @@ static void plan_bands(HeadPlan& plan, int rows, int units, int limit) {
     plan.part0[i] = part;
     first += b;
     part += b * plan.block_rows * plan.strips[i];
+  }
+  plan.box = 128;
+  if (!in_pairs(rows)) {      // one band, for a launch of so few rows is one block
+    plan.box = plan.tile[0] = tile_of(plan.width[0], K);
+    const int fit = HS_RING / ((box_rows<false>(rows) + plan.box) * HS_BK * 2);
+    plan.stages = fit < HS_STAGES ? fit : HS_STAGES;
   }
 }
 // Whether a row's strips are wide enough that what they note pays for a memset ahead of the kernel. 5 and 20
@@ -666,7 +691,7 @@ MB_EXPORT long long mb_head_scores_scratch(int rows, int limit, int top, int sms
   for (const int n : {rows < most ? 0 : most, rows % most}) {
     if (n == 0) continue;
     HeadPlan plan;
-    plan_bands(plan, n, head_units(in_pairs(n), sms), limit);
+    plan_bands(plan, n, head_units(in_pairs(n), sms), limit, 0);
     if (parts_of(plan) > parts) parts = parts_of(plan);
   }
   const int one = rows < most ? rows : most;
@@ -689,16 +714,15 @@ MB_EXPORT int mb_head_scores(const void* A, int lda, const void* W, int rows, in
     MB_FAIL("mb_head_scores: %lld bytes of scratch", scratch_bytes);
   const int form = head_form(top), most = HS_BLOCKS * block_rows_of(true);
   cudaStream_t s = (cudaStream_t)stream;
-  CUtensorMap tmB;
-  if (!mb_make_map_bf16(&tmB, W, limit, K, K, 128, "mb_head_scores weight")) return -1;
   for (int r0 = 0; r0 < rows; r0 += most) {
     const int n = rows - r0 < most ? rows - r0 : most;
     const bool pair = in_pairs(n);
     if (cudaError_t e = allow_smem(pair, form)) MB_FAIL("mb_head_scores: %s", cudaGetErrorString(e));
     const __nv_bfloat16* a = (const __nv_bfloat16*)A + (size_t)r0 * lda;
     HeadPlan plan = {};
-    plan_bands(plan, n, head_units(pair, sms), limit);
-    CUtensorMap tmA;
+    plan_bands(plan, n, head_units(pair, sms), limit, K);
+    CUtensorMap tmA, tmB;
+    if (!mb_make_map_bf16(&tmB, W, limit, K, K, plan.box, "mb_head_scores weight")) return -1;
     const int box = pair ? box_rows<true>(n) : box_rows<false>(n);
     if (!mb_make_map_bf16(&tmA, a, n, K, lda, box, "mb_head_scores input")) return -1;
     const size_t parts = parts_of(plan);

@@ -19,16 +19,15 @@ from .linear import Linear, Pending
 SCORE_BAND = 1 << 28
 
 
-def scores_through_memory(rows: int, width: int, vocab: int, top: int) -> bool:
-    """Whether the logits of these rows are better stored. Of few wide rows: the product of few rows
-    streams the head a little faster (1 row of 2,560 values before 151,936 ids 143 us against 154, 32 rows
-    150 against 154). Of many alternatives: the fused kernel keeps lists of its own for every strip
-    of a row, while the stored logits of few rows are read from L2. Fused | stored, us: 20 alternatives of
-    151,936 ids, 32 rows of 1,024 values 93 | 88, 96 rows 94 | 113; of 32,000 ids, 257 rows 72 | 57, 512
-    rows 80 | 70, 1,001 rows 97 | 117; 32 alternatives of 151,936, 128 rows 129 | 117, 257 rows 201 | 201,
-    of 2,560 values 291 | 330. With 8 or fewer the fused kernel is as quick from the first row on: 5
-    alternatives, 8 rows of 1,024 values 83 | 84, 128 rows 86 | 109."""
-    return (rows <= 32 and width >= 2048) or rows * vocab <= (top - 8) << 20
+def scores_through_memory(rows: int, vocab: int, top: int) -> bool:
+    """Whether the logits of these rows are better stored: those of few rows with many alternatives. The
+    fused kernel keeps lists of its own for every strip of a row, while the stored logits of few rows are
+    read from L2. Fused | stored, us: 20 alternatives of 151,936 ids, 32 rows of 1,024 values 93 | 88, 96
+    rows 94 | 113; of 32,000 ids, 257 rows 72 | 57, 512 rows 80 | 70, 1,001 rows 97 | 117; 32
+    alternatives of 151,936, 128 rows 129 | 117, 257 rows 201 | 201, of 2,560 values 291 | 330. With 8 or
+    fewer the fused kernel is as quick from the first row on: 5 alternatives, 8 rows of 1,024 values
+    78 | 84, of 4,096 214 | 223, 128 rows of 1,024 84 | 109."""
+    return rows * vocab <= (top - 8) << 20
 
 
 class TokenEmbedding(Part):
@@ -105,7 +104,7 @@ class LmHead(Part):
         if rows == 0:
             return out
         tokens = tokens.contiguous()
-        if (self.linear.fast is not None and not scores_through_memory(rows, self.hidden, limit, top)
+        if (self.linear.fast is not None and not scores_through_memory(rows, limit, top)
                 and K.head_scores_supported(h, weight)):
             K.head_scores(h, weight, limit, self.scale, self.softcap, tokens, top, out, rt.error_word)
             return out
