@@ -461,7 +461,7 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         const int strips = plan.strips[walk.band];
         const size_t part =
             plan.part0[walk.band] + ((size_t)walk.block * block_rows_of(PAIR) + in_block) * strips + walk.strip;
-        mass[part] = {m, s, t};
+        mass[part] = {m, s - 1.f, t};      // as rest_join takes it
         list.write(keys + part * top, top);
       }
     }
@@ -498,17 +498,20 @@ head_join_kernel(const __grid_constant__ HeadPlan plan, const Mass* __restrict__
   float most = -INFINITY;
 #pragma unroll
   for (int i = 0; i < HS_STRIPS / 32; ++i) {
-    v[i] = lane + 32 * i < strips ? mass[part + lane + 32 * i] : mass_none();
+    v[i] = lane + 32 * i < strips ? mass[part + lane + 32 * i] : rest_none();
     most = fmaxf(most, v[i].m);
   }
   most = warp_max(most);
   Mass all = {most, 0.f, 0.f};
+  int tops = -1;
 #pragma unroll
   for (int i = 0; i < HS_STRIPS / 32; ++i) {
-    const Mass p = mass_over(v[i], most);
+    const bool top_one = v[i].m == most;
+    const Mass p = top_one ? v[i] : mass_over({v[i].m, v[i].s + 1.f, v[i].t}, most);
     all.s += p.s, all.t += p.t;
+    tops += __popc(__ballot_sync(0xffffffffu, top_one));
   }
-  all.s = warp_sum(all.s);
+  all.s = warp_sum(all.s) + (float)tops;
   all.t = warp_sum(all.t);
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncwarp();

@@ -69,7 +69,7 @@ struct ScShared {
   alignas(16) uint32_t place[SC_ROOM];      // of the keys held, in order, and of those that passed the bar
   uint32_t id[SC_ROOM];                     // and their ids
   TopKey sorted[MB_SCORES_TOP], pick[SC_WARPS];
-  int taken[MB_SCORES_TOP], passed[3], equal[2];
+  int taken[MB_SCORES_TOP], passed[3], equal[2], tops[SC_WARPS];
   float most[SC_WARPS], s[SC_WARPS], t[SC_WARPS];
   // of the cluster's first CTA: every CTA's part
   Mass mass[SC_CLUSTER];
@@ -173,7 +173,8 @@ __device__ __noinline__ void sc_pick(const float* __restrict__ x, int base, int 
   __syncthreads();
 }
 
-// What a CTA finds in its part of a row, x[0 .. n) with ids from id0 on: the mass (every thread has it),
+// What a CTA finds in its part of a row, x[0 .. n) with ids from id0 on: the mass (every thread has it, S - 1 in
+// place of S),
 // and in sh.sorted the greatest `top` keys in order, 0 where there are no more finite values.
 //
 // The first round sets a bar that few values pass and the `top` greatest do: with every warp's ceil(top / 8)
@@ -263,14 +264,19 @@ __device__ __forceinline__ Mass sc_part(const float* __restrict__ x, int n, int 
   float most = sh.most[0];
 #pragma unroll
   for (int w = 1; w < SC_WARPS; ++w) most = fmaxf(most, sh.most[w]);
-  mine = mass_over(mine, most);
+  // (a thread's sums have its own greatest value's 1 in them: see rest_join)
+  const unsigned tops = __ballot_sync(0xffffffffu, mine.m == most);
+  if (lane == 0) sh.tops[warp] = __popc(tops);
+  mine = mine.m == most ? Mass{most, mine.s - 1.f, mine.t} : mass_over(mine, most);
   mine.s = warp_sum(mine.s);
   mine.t = warp_sum(mine.t);
   if (lane == 0) sh.s[warp] = mine.s, sh.t[warp] = mine.t;
   __syncthreads();
   mine = {most, 0.f, 0.f};
+  int all = -1;
 #pragma unroll
-  for (int w = 0; w < SC_WARPS; ++w) mine.s += sh.s[w], mine.t += sh.t[w];
+  for (int w = 0; w < SC_WARPS; ++w) mine.s += sh.s[w], mine.t += sh.t[w], all += sh.tops[w];
+  mine.s += (float)all;
   return mine;
 }
 
@@ -320,10 +326,10 @@ token_scores_kernel(const float* __restrict__ logits, size_t stride, int V, int 
   }
   if (threadIdx.x >= 32) return;
   const int lane = threadIdx.x;
-  Mass all = lane < parts ? sh.mass[lane] : mass_none();
+  Mass all = lane < parts ? sh.mass[lane] : rest_none();
 #pragma unroll
   for (int o = SC_CLUSTER / 2; o > 0; o >>= 1)
-    all = mass_join(all, {__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.s, o),
+    all = rest_join(all, {__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.s, o),
                           __shfl_xor_sync(0xffffffffu, all.t, o)});
   const TopKey mine = TOP && lane < top ? sh.sorted[lane] : 0;
   all = {__shfl_sync(0xffffffffu, all.m, 0), __shfl_sync(0xffffffffu, all.s, 0), __shfl_sync(0xffffffffu, all.t, 0)};

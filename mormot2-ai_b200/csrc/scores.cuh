@@ -32,11 +32,15 @@ __device__ __forceinline__ Mass mass_over(Mass a, float m) {
   const float d = a.m - m, e = a.m == -INFINITY ? 0.f : expf(d);
   return {m, e * a.s, e > 0.f ? e * fmaf(d, a.s, a.t) : e * a.s};
 }
-__device__ __forceinline__ Mass mass_join(Mass a, Mass b) {
-  const float m = fmaxf(a.m, b.m);
-  a = mass_over(a, m);
-  b = mass_over(b, m);
-  return {m, a.s + b.s, a.t + b.t};
+// Parts that are joined bring S - 1 instead of S: most rows have one value far above all others, and its 1 in
+// a sum of 32 bits would round away what ln S = log1p(S - 1) is made of (a log probability of -0.0104 was off by
+// 3.5e-7).
+__device__ __forceinline__ Mass rest_none() { return {-INFINITY, -1.f, 0.f}; }
+__device__ __forceinline__ Mass rest_join(Mass a, Mass b) {
+  const bool first = a.m >= b.m;
+  const Mass top = first ? a : b, low = first ? b : a;
+  const Mass less = mass_over({low.m, low.s + 1.f, low.t}, top.m);
+  return {top.m, top.s + less.s, top.t + less.t};
 }
 
 // N values onto the sums over a maximum `m` that is final (0 stands for -infinity): s += sum e^(x - m),
@@ -56,18 +60,6 @@ template <int N> __device__ __forceinline__ void mass_add(const float* x, float 
   const f32_pair a = pair_add(ps[0], ps[1]), b = pair_add(pt[0], pt[1]);
   s += pair_half(a, 0) + pair_half(a, 1);
   t += pair_half(b, 0) + pair_half(b, 1);
-}
-
-__device__ __forceinline__ Mass mass_warp(Mass v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Mass w;
-    w.m = __shfl_xor_sync(0xffffffffu, v.m, o);
-    w.s = __shfl_xor_sync(0xffffffffu, v.s, o);
-    w.t = __shfl_xor_sync(0xffffffffu, v.t, o);
-    v = mass_join(v, w);
-  }
-  return v;
 }
 
 // A value and its id as one number: the greater value first, the lowest id among equals, -0 equal to
@@ -93,16 +85,16 @@ struct ScoreOut {
   float* top_logprobs;
 };
 
-// What a warp makes of a row's joined mass, the given token's logit (a NaN where there is none) and the
+// What a warp makes of a row's joined mass (S - 1 in place of S), the given token's logit (a NaN where there is none) and the
 // greatest values in order, lane j the j-th's key (0 where there are no more). What is left then are
 // values of -infinity (or NaNs, in a row whose numbers are NaN anyway): the lowest ids that are not listed.
 __device__ __forceinline__ void finish_row(Mass v, float given, TopKey key, int top, int row,
                                            const ScoreOut& out) {
   const int lane = threadIdx.x & 31;
-  const float ln_s = logf(v.s);
+  const float ln_s = log1pf(v.s);
   if (lane == 0) {
     out.logprobs[row] = given - v.m - ln_s;
-    const float h = ln_s - v.t / v.s;
+    const float h = ln_s - v.t / (1.f + v.s);
     out.entropy[row] = h < 0.f ? 0.f : h;
   }
   if (top == 0) return;

@@ -159,6 +159,28 @@ def test_the_same_again_on_streams_and_in_graphs():
             assert torch.equal(a, b)
 
 
+def test_one_token_nearly_certain():
+    """Rows whose likeliest token has all but some 1e-2 to 1e-4: ln S is that small, and what the sums lose of
+    it is what they round beside that token's 1. Only its own thread adds to it (10 values of a thread, four
+    sums of them, joined: 12 additions), each off by at most 2^-24, 2^-23 / sqrt(12) in the mean; the rest is
+    joined apart from the 1."""
+    rng = np.random.default_rng(41)
+    rows, V = 700, 20000
+    x = rng.standard_normal((rows, V)).astype(np.float32)
+    best = rng.integers(0, V, rows).astype(np.int32)
+    x[np.arange(rows), best] = rng.uniform(15.0, 19.0, rows).astype(np.float32)
+    for n in (1, 4, rows):
+        off = []
+        for a in range(0, rows, n if n > 1 else 7):
+            part = slice(a, a + n)
+            got = token_scores(torch.from_numpy(x[part]).to(DEV), torch.from_numpy(best[part]).to(DEV), 3)
+            d = x[part].astype(np.float64) - x[part].max(1, keepdims=True)
+            off.append(got.logprobs.double().cpu().numpy() + np.log1p(np.exp(np.sort(d, 1)[:, :-1]).sum(1)))
+        off = np.concatenate(off)
+        rounds = 12 if n < rows else 12 + V // 256 // 4       # many rows: a row is one CTA's, in rounds
+        assert np.sqrt((off ** 2).mean()) <= np.sqrt(rounds / 12) * 2.0 ** -23, n
+
+
 # ---------------------------------------------------------------------------- the head
 @pytest.fixture(params=["as it chooses", "fused"])
 def form(request, monkeypatch):
