@@ -168,9 +168,11 @@ template <> struct TopList<0> {
   __device__ __forceinline__ void write(TopKey*, int) const {}
 };
 
-// 32 columns of this thread's lane
+// 32 columns of this thread's lane. The load is one of a whole warp, and the code between two of them leaves lanes
+// behind (rows that are not there, values that go into lists): they come together first.
 __device__ __forceinline__ void load32(uint32_t taddr, float* x) {
   uint32_t a[16], b[16];
+  __syncwarp();
   TMEM_LD16(a, 0);
   TMEM_LD16(b, 16);
   TMEM_HOLD16("tcgen05.wait::ld.sync.aligned;", a);
@@ -268,6 +270,7 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   if (warp == 1) {
     if (PAIR) tmem_alloc_pair(slot, 512); else tmem_alloc(slot, 512);
   }
+  __syncwarp();      // the cluster's barrier takes whole warps too
   tc_fence_before_sync();
   if (PAIR) cluster_sync_all(); else __syncthreads();
   tc_fence_after_sync();
@@ -467,6 +470,7 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     }
   }
   // neither CTA of a pair leaves while the other may still read its shared memory or signal its barriers
+  __syncwarp();
   tc_fence_before_sync();
   if (PAIR) cluster_sync_all(); else __syncthreads();
   if (warp == 1) {
