@@ -51,6 +51,14 @@ class Entry:
     given: Optional[Sequence[int]] = None
 
 
+def _check_places(e: Entry) -> None:
+    """Refuses wanted places in an array that is no list: rows of several would be as many places more
+    than the caller counts."""
+    w = e.want
+    if isinstance(w, np.ndarray) and (w.ndim == 0 or w.size != len(w)):
+        raise InferError(f"slot {e.slot}: wanted places in an array of shape {w.shape}, not in a list")
+
+
 @dataclass
 class _Scoring:
     """What a step gives instead of logits: scores of these tokens, one a wanted row."""
@@ -258,6 +266,7 @@ class Engine:
         below = candidates(self.vocab_size, vocab_limit)
         placed, given = [], []
         for e in entries:
+            _check_places(e)
             g, want = e.given, e.want
             if g is None:
                 if want is not None:
@@ -304,6 +313,7 @@ class Engine:
                     raise InferError(f"slot {e.slot}: token {int(tokens[bad][0])} is outside "
                                      f"the vocabulary of {self.vocab_size}")
             if isinstance(e.want, np.ndarray):
+                _check_places(e)
                 # (64 bits: added to a first row, narrower integers would wrap)
                 want = e.want.astype(np.int64).reshape(-1)
                 outside = want.size and not 0 <= want.min() <= want.max() < len(tokens)

@@ -1,0 +1,83 @@
+"""Steps that score, without a GPU: an engine whose model is a table of logits by token, on the host."""
+from types import SimpleNamespace
+
+import numpy as np
+import pytest
+import torch
+
+from mormot2_ai_b200 import Engine, Entry, InferError
+from mormot2_ai_b200.cache.pages import CacheBook, GroupPlan
+from mormot2_ai_b200.sampling import Scores
+
+VOCAB, SLOTS, CONTEXT = 50, 4, 1024
+
+
+class TableModel:
+    """The logits behind a token are a row of a table and do not depend on what stood before."""
+
+    def __init__(self):
+        self.logp = torch.randn((VOCAB, VOCAB), generator=torch.Generator().manual_seed(1)).log_softmax(1)
+
+    def forward(self, ctx, cache, on_state=None, score=None):
+        if not ctx.n_want:
+            return None
+        x = self.logp[ctx.wanted]
+        if score is None:
+            return x
+        given, top, limit = score
+        assert given.shape == (ctx.n_want,)
+        values, ids = x.topk(top, dim=1)
+        return Scores(x.gather(1, given.long()[:, None])[:, 0], -(x.exp() * x).sum(1), ids.to(torch.int32),
+                      values)
+
+
+class Buffers:
+    copied_bytes = 0
+
+    def fill(self, seqs, longest_first=False):
+        wanted = [int(s[2][w]) for s in seqs for w in s[3]]
+        return SimpleNamespace(T=sum(len(s[2]) for s in seqs), B=len(seqs), n_want=len(wanted),
+                               wanted=wanted, entry_slots=None, decode=all(len(s[2]) == 1 for s in seqs))
+
+
+def table_engine(prefill_chunk=64, max_step_tokens=100):
+    eng = Engine.__new__(Engine)
+    plans = [GroupPlan(1, 16, 0, [0], 64, CONTEXT // 64, 0)]
+    eng.book = CacheBook(plans, SLOTS, CONTEXT)
+    eng.cache = SimpleNamespace(map_grown=lambda *lists: None, reset_state=lambda slot: None)
+    eng.rt = SimpleNamespace(device=torch.device("cpu"))
+    eng.buffers, eng.model = Buffers(), TableModel()
+    eng.vocab_size, eng.max_context, eng.max_slots = VOCAB, CONTEXT, SLOTS
+    eng.prefill_chunk, eng.max_step_tokens = prefill_chunk, max_step_tokens
+    eng.has_state, eng.state_ok, eng.ids = False, [True] * SLOTS, [[] for _ in range(SLOTS)]
+    eng.run = eng.on_state = None
+    eng.use_graphs, eng.sort_from, eng.passes = False, 1 << 30, 0
+    return eng
+
+
+def text(n, seed=0):
+    return np.random.default_rng(seed).integers(0, VOCAB, n).tolist()
+
+
+@pytest.mark.parametrize("places", [np.array([[0, 1, 2], [3, 4, 5]]), np.array(3), np.zeros((3, 0), int),
+                                    np.zeros((1, 2, 2), int)])
+def test_places_that_are_no_list_are_refused(places):
+    """Before any page is reserved, and whether or not the count of rows is that of the given tokens."""
+    eng = table_engine()
+    slot = eng.open()
+    for n in (8, 200):
+        with pytest.raises(InferError, match="shape"):
+            eng.step([Entry(slot, text(n), places)])
+        for given in ([1, 2], [1] * 6, [1], []):
+            with pytest.raises(InferError, match="shape"):
+                eng.score([Entry(slot, text(n), places, given)], top=2)
+    assert eng.length(slot) == 0 and eng.book.held_pages(0) == 0 and eng.passes == 0
+
+
+def test_places_in_rows_of_one():
+    """A column of places is as many rows as places."""
+    eng = table_engine()
+    slot, t = eng.open(), text(150)
+    x = eng.step([Entry(slot, t, np.array([[7], [149]]))])
+    assert torch.equal(x, eng.model.logp[[t[7], t[149]]])
+    assert eng.step([Entry(slot, [1], np.zeros((0, 3), int))]) is None
