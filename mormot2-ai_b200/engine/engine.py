@@ -364,7 +364,9 @@ class Engine:
                 self.last_h2d_bytes += self.buffers.copied_bytes
                 self.last_slots = ctx.entry_slots
                 if scoring is not None:
-                    self._score_pass(ctx, scoring, given, dest, out)
+                    # one pass brings the rows as they are wanted; several sort an entry's places
+                    whole = len(passes) == 1 or dest == list(range(n_want))
+                    self._score_pass(ctx, scoring, given, None if whole else dest, out)
                     self.passes += 1
                     continue
                 logits = self._forward(ctx)
@@ -411,9 +413,10 @@ class Engine:
         return logits, shares, e0.elapsed_time(e1)
 
     def _score_pass(self, ctx: StepContext, scoring: _Scoring, given: torch.Tensor,
-                    dest: List[int], out: Scores) -> None:
-        """One pass whose wanted rows are scored: rows ``dest`` of ``out``."""
-        whole = ctx.n_want == out.logprobs.shape[0]      # a pass of all rows brings them in order
+                    dest: Optional[List[int]], out: Scores) -> None:
+        """One pass whose wanted rows are scored: rows ``dest`` of ``out`` (None: all of them, in
+        order)."""
+        whole = dest is None
         places = None
         if not whole and ctx.n_want:
             places = torch.tensor(dest, dtype=torch.long, device=given.device)

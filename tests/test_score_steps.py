@@ -81,3 +81,27 @@ def test_places_in_rows_of_one():
     x = eng.step([Entry(slot, t, np.array([[7], [149]]))])
     assert torch.equal(x, eng.model.logp[[t[7], t[149]]])
     assert eng.step([Entry(slot, [1], np.zeros((0, 3), int))]) is None
+
+
+@pytest.mark.parametrize("cut", [dict(), dict(max_step_tokens=64), dict(prefill_chunk=7, max_step_tokens=30),
+                                 dict(prefill_chunk=1000, max_step_tokens=1000)])
+@pytest.mark.parametrize("places", [[99, 70], [99, 70, 99], [70, 99], [30, 0, 7], list(range(99, 63, -1)),
+                                    [5, 5, 2, 99, 0], [99], []])
+def test_places_in_any_order(places, cut):
+    """All wanted rows in one of a step's several passes, or spread over them, one text or several."""
+    eng = table_engine(**cut)
+    for others in ([], [[3, 1]], [[], [0]]):
+        ids = [text(100)] + [text(5, seed=9 + i) for i in range(len(others))]
+        wants = [places] + others
+        given = [text(len(w), seed=31 + i) for i, w in enumerate(wants)]
+        for kind in (list, np.array):
+            slots = [eng.open() for _ in ids]
+            got = eng.score([Entry(s, t, kind(w) if w else w, g)
+                             for s, t, w, g in zip(slots, ids, wants, given)], top=4)
+            rows = eng.model.logp[[t[w] for t, want in zip(ids, wants) for w in want]]
+            tokens = torch.tensor([g for one in given for g in one], dtype=torch.long)
+            assert torch.equal(got.logprobs, rows.gather(1, tokens[:, None])[:, 0])
+            values, order = rows.topk(4, dim=1)
+            assert torch.equal(got.top_ids, order.to(torch.int32)) and torch.equal(got.top_logprobs, values)
+            for s in slots:
+                eng.close(s)
