@@ -10,6 +10,7 @@ from typing import Dict, List, Optional
 import torch
 
 from .. import kernels as K
+from ..errors import InferError
 from ..sampling.scores import Scores, check_score
 from .base import EMBEDDINGS, ENTRIES, HEADS, Part, TensorNeed
 from .linear import Linear, Pending
@@ -94,6 +95,8 @@ class LmHead(Part):
             with K.on_device_of(h):
                 return self.score(h, tokens, top, vocab_limit)
         rows, weight, rt = h.shape[0], self.linear.weight, self.linear.rt
+        if weight.get_device() != h.get_device():
+            raise InferError(f"scores: the head's input is on {h.device}, its weight on {weight.device}")
         if not self.hidden <= h.stride(0) < 1 << 31:      # one row many times, or rows 4 GiB apart
             h = h.clone(memory_format=torch.contiguous_format)
         floats = h if h.dtype == torch.float32 else rt.workspace

@@ -5,8 +5,10 @@ import numpy as np
 import pytest
 import torch
 
-from mormot2_ai_b200 import Engine, Entry, InferError
+from mormot2_ai_b200 import Engine, Entry, InferError, PartSpec
+from mormot2_ai_b200 import kernels as K
 from mormot2_ai_b200.cache.pages import CacheBook, GroupPlan
+from mormot2_ai_b200.parts import HEADS
 from mormot2_ai_b200.sampling import Scores
 
 VOCAB, SLOTS, CONTEXT = 50, 4, 1024
@@ -105,3 +107,14 @@ def test_places_in_any_order(places, cut):
             assert torch.equal(got.top_ids, order.to(torch.int32)) and torch.equal(got.top_logprobs, values)
             for s in slots:
                 eng.close(s)
+
+
+def test_a_head_on_another_device(monkeypatch):
+    """Rows beside a head whose weight another device holds: refused before anything is launched."""
+    head = HEADS.build(PartSpec("lm_head", {"name": "w", "tied": False, "vocab_size": 50, "hidden_size": 8}))
+    weight = SimpleNamespace(get_device=lambda: 1, device="cuda:1")
+    head.linear = SimpleNamespace(weight=weight, rt=None)
+    monkeypatch.setattr(K, "elsewhere", lambda device: False)       # the rows' device is the current one
+    h, tokens = torch.zeros(3, 8, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(InferError, match="weight on cuda:1"):
+        head.score(h, tokens, 2)
