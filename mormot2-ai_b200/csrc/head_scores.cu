@@ -340,7 +340,9 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     while (walk.next_strip()) {
       const int in_block = (int)rank * 128 + lane_row, row = walk.row0() + in_block;
       const int token = row < rows ? tokens[row] : -1;
-      float m = -INFINITY, s = 0.f, t = 0.f;     // the row's mass
+      // The row's mass, S - 1 in place of S from the first value on: beside the likeliest token's 1 a tile of
+      // less than 2^-24 would be lost, and of a nearly certain token all others are such tiles.
+      float m = -INFINITY, s = 0.f, t = 0.f;
       TopList<N> list;
       list.clear(top);
       int seen = 0;                              // tiles of the strip
@@ -416,14 +418,17 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll
             for (int g = 0; g < 4; ++g) groups[g] = fmaxf(groups[g], eights[g]);
           }
-          if (most > m) {
-            const Mass row_part = mass_over({m, s, t}, most), tile_part = mass_over({m, tile_s, tile_t}, most);
+          const bool moved = most > m;
+          if (moved) {
+            const Mass row_part = mass_over({m, s + 1.f, t}, most), tile_part = mass_over({m, tile_s, tile_t}, most);
             m = most;
             s = row_part.s, t = row_part.t;
             tile_s = tile_part.s, tile_t = tile_part.t;
           }
           const float at = m == -INFINITY ? 0.f : m;
-          mass_add<32>(x, at, tile_s, tile_t);
+          float piece = 0.f;                     // where the maximum is new, its 1 is in here
+          mass_add<32>(x, at, piece, tile_t);
+          tile_s += moved ? piece - 1.f : piece;
           const unsigned off = (unsigned)token - (unsigned)id0;
           if (__any_sync(0xffffffffu, off < (unsigned)n)) {
 #pragma unroll
@@ -464,7 +469,7 @@ head_scores_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         const int strips = plan.strips[walk.band];
         const size_t part =
             plan.part0[walk.band] + ((size_t)walk.block * block_rows_of(PAIR) + in_block) * strips + walk.strip;
-        mass[part] = {m, s - 1.f, t};      // as rest_join takes it
+        mass[part] = {m, m == -INFINITY ? s - 1.f : s, t};      // as rest_join takes it (no value: no 1 either)
         list.write(keys + part * top, top);
       }
     }
