@@ -23,7 +23,7 @@ from .config.registry import read_config_json
 from .engine.engine import Engine, Entry
 from .engine.generate import EngineStepper, Outcome, Request, generate, plan_batches
 from .errors import InferError
-from .sampling.scores import TokenScore
+from .sampling.scores import TokenScore, candidates, check_top
 from .sampling.settings import Sampling, sampling_from_config
 
 
@@ -118,6 +118,8 @@ class LlmClient:
         log probability after the tokens before it, the entropy there and the ``top`` (0 to 32) most
         probable alternatives. Sequences run together as the cache allows."""
         texts = [[int(t) for t in s] for s in sequences]
+        below = candidates(self.engine.vocab_size, self.vocab_limit)
+        check_top(top, below)
         for i, t in enumerate(texts):
             if not t:
                 raise InferError(f"sequence {i}: empty")
@@ -128,6 +130,9 @@ class LlmClient:
             if bad:
                 raise InferError(f"sequence {i}: token {bad[0]} is outside the vocabulary of "
                                  f"{self.engine.vocab_size}")
+            bad = [a for a in t[1:] if a >= below]      # the first token is fed alone
+            if bad:
+                raise InferError(f"sequence {i}: token {bad[0]} to score is outside the vocabulary of {below}")
         out = [TextScore([]) for _ in texts]
         fed = [i for i, t in enumerate(texts) if len(t) > 1]
         pools = [(p.n_pages, p.ring_pages) for p in self.engine.plans]

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from mormot2_ai_b200 import Engine, Entry, InferError, PartSpec
+from mormot2_ai_b200 import Engine, Entry, InferError, LlmClient, PartSpec
 from mormot2_ai_b200 import kernels as K
 from mormot2_ai_b200.cache.pages import CacheBook, GroupPlan
 from mormot2_ai_b200.parts import HEADS
@@ -118,3 +118,40 @@ def test_a_head_on_another_device(monkeypatch):
     h, tokens = torch.zeros(3, 8, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int32)
     with pytest.raises(InferError, match="weight on cuda:1"):
         head.score(h, tokens, 2)
+
+
+def table_client(max_batch=2, vocab_limit=None):
+    client = LlmClient.__new__(LlmClient)
+    client.engine = table_engine()
+    client.engine.plans = client.engine.book.plans
+    client.engine.rt.check = lambda: None
+    client.max_batch, client.vocab_limit = max_batch, vocab_limit
+    return client
+
+
+def test_texts_in_batches():
+    client = table_client()
+    texts = [text(n, seed=n) for n in (3, 1, 150, 2, 90)]
+    got = client.score(texts, top=2)
+    for t, s in zip(texts, got):
+        want = client.engine.model.logp[t[:-1]].gather(1, torch.tensor(t[1:]).long()[:, None])[:, 0]
+        assert [x.logprob for x in s.tokens] == want.tolist()
+        assert all(len(x.alternatives) == 2 for x in s.tokens)
+    assert client.engine.book.slots.free == SLOTS
+
+
+@pytest.mark.parametrize("texts,top,match", [
+    ([[1, 2], [3, 4], [5, 6], [7, 40]], 1, "sequence 3: token 40"),      # to score, but no candidate
+    ([[1, 2], [3, 4], [5, 6], [50, 4]], 1, "sequence 3: token 50"), ([[1, 2], [3, -1]], 1, "sequence 1: token -1"),
+    ([[1, 2], []], 1, "sequence 1: empty"), ([[1], [2]], 33, "33 alternatives"), ([[1]], -1, "alternatives"),
+    ([[1, 2]], 31, "31 alternatives"), ([[1, 2]], True, "alternatives")])
+def test_texts_are_refused_before_any_runs(texts, top, match):
+    client = table_client(vocab_limit=30)
+    with pytest.raises(InferError, match=match):
+        client.score(texts, top=top)
+    assert client.engine.passes == 0 and client.engine.book.slots.free == SLOTS
+
+
+def test_a_first_token_is_fed_and_not_scored():
+    client = table_client(vocab_limit=30)
+    assert [len(s.tokens) for s in client.score([[45, 3, 29], [45]], top=1)] == [2, 0]
