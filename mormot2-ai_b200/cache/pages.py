@@ -159,11 +159,6 @@ class CacheBook:
         n = pages_for(length)
         return min(n, plan.ring_pages) if plan.ring_pages else n
 
-    def missing(self, slot: int, new_length: int) -> List[int]:
-        """How many pages each group still has to map for the slot to hold new_length."""
-        return [max(0, self.entries_needed(g, new_length) - len(self.pages[g][slot]))
-                for g in range(len(self.plans))]
-
     def reserve(self, requests: List[Tuple[int, int]]) -> List[List[Tuple[int, int, int]]]:
         """Maps the pages that the slots need to reach their new lengths:
         ``requests = [(slot, new_length)]``. All or nothing: if a pool runs out, nothing is
