@@ -17,8 +17,8 @@
 // 4,096 values 804 us with the tensor pipe 98 % active, weights read once, 1.30 GB; 2,048 rows again and
 // again 1.35 PFLOP/s under the power cap, on rows of few bits 1.53). Below that the four warps that read
 // tensor memory: some 550 cycles for 32 ids of a row (the exponentials alone take 256), and the lists, some
-// 110 instructions a value that goes in (1,024 values a row, 1,001 rows: 212 us without alternatives, 228 with 5,
-// 300 with 20). Up to 128 rows the head's bytes (24 rows of 1,024 values: 52 us, 6.0 TB/s; of 4,096:
+// 110 instructions a value that goes in (1,024 values a row, 1,001 rows: 195 us without alternatives, 215 with 5,
+// 270 with 20). Up to 128 rows the head's bytes (24 rows of 1,024 values: 52 us, 6.0 TB/s; of 4,096:
 // 188, 6.6; 128 rows 55 and 214).
 // Taken back: two such warps a quarter of the lanes, a tile each in turn (their lists see half the ids each,
 // and together nearly twice the new values: 501 us, 656 with 20); ids in a log beside the values in

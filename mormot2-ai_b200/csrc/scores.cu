@@ -173,9 +173,8 @@ __device__ __noinline__ void sc_pick(const float* __restrict__ x, int base, int 
   __syncthreads();
 }
 
-// What a CTA finds in its part of a row, x[0 .. n) with ids from id0 on: the mass (every thread has it, S - 1 in
-// place of S),
-// and in sh.sorted the greatest `top` keys in order, 0 where there are no more finite values.
+// What a CTA finds in its part of a row, x[0 .. n) with ids from id0 on: the mass (every thread has it, S - 1
+// in place of S), and in sh.sorted the greatest `top` keys in order, 0 where there are no more finite values.
 //
 // The first round sets a bar that few values pass and the `top` greatest do: with every warp's ceil(top / 8)
 // greatest threads there are `top`, so the least of these threads' greatest values is one (of 10,240 values

@@ -85,9 +85,9 @@ struct ScoreOut {
   float* top_logprobs;
 };
 
-// What a warp makes of a row's joined mass (S - 1 in place of S), the given token's logit (a NaN where there is none) and the
-// greatest values in order, lane j the j-th's key (0 where there are no more). What is left then are
-// values of -infinity (or NaNs, in a row whose numbers are NaN anyway): the lowest ids that are not listed.
+// What a warp makes of a row's joined mass (S - 1 in place of S), the given token's logit (a NaN where there
+// is none) and the greatest values in order, lane j the j-th's key (0 where there are no more). What is left
+// then are values of -infinity (or NaNs, in a row whose numbers are NaN anyway): the lowest ids that are not listed.
 __device__ __forceinline__ void finish_row(Mass v, float given, TopKey key, int top, int row,
                                            const ScoreOut& out) {
   const int lane = threadIdx.x & 31;

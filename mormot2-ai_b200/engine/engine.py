@@ -261,7 +261,8 @@ class Engine:
         to its sequence, as ``step`` does, and returns the scores of its ``given`` tokens at the
         wanted places, in the order of the entries and of their ``want``: log probabilities,
         entropy and the ``top`` (up to 32) most probable alternatives, among the ids below
-        ``vocab_limit``. The logits of many rows are never stored."""
+        ``vocab_limit``. The logits of many rows are never stored. (Unlike a step it waits for the device:
+        the given tokens are copied from ordinary memory.)"""
         top = check_top(top, candidates(self.vocab_size, vocab_limit))
         below = candidates(self.vocab_size, vocab_limit)
         placed, given = [], []

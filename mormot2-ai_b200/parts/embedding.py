@@ -25,7 +25,8 @@ def scores_through_memory(rows: int, vocab: int, top: int) -> bool:
     fused kernel keeps lists of its own for every strip of a row, while the stored logits of few rows are
     read from L2. Fused | stored, us: 20 alternatives of 151,936 ids, 32 rows of 1,024 values 93 | 88, 96
     rows 94 | 113; of 32,000 ids, 257 rows 72 | 57, 512 rows 80 | 70, 1,001 rows 97 | 117; 32
-    alternatives of 151,936, 128 rows 129 | 117, 257 rows 201 | 201, of 2,560 values 291 | 330. With 8 or
+    alternatives of 151,936, 128 rows 129 | 117, 257 rows 201 | 201, of 2,560 values 291 | 330. (No bound on the
+    values alone has both the 96 rows and the 512 on their quicker side; the 512 are not.) With 8 or
     fewer the fused kernel is as quick from the first row on: 5 alternatives, 8 rows of 1,024 values
     78 | 84, of 4,096 214 | 223, 128 rows of 1,024 84 | 109."""
     return rows * vocab <= (top - 8) << 20
